@@ -12,6 +12,7 @@ check, mirroring the reference crate's encoder seam:
     .encode_batch(sub, cu)     varlen batch (one utterance per segment)
     .linear_lut4(...)          Ctx::gemm_f32 with a low-bit weight + add_bias
                                (src/encoder.rs:1039-1100)
+    KvCache, sample            text generation on torch tensors (textgen.py)
 
 There is no CPU fallback: if the shared library is missing or cannot load,
 every entry point raises.
@@ -98,6 +99,10 @@ def lib() -> ctypes.CDLL:
         "b3_mel": (c_i, [c_p, c_p, c_p, c_i, c_p, c_p, c_u]),
         "b3_subsample": (c_i, [c_p, c_p, c_p, c_p, c_i, c_p, c_p, c_u]),
         "b3_mel_filters": (c_i, [c_p]),
+        "b3_kv_append": (c_i, [c_p] * 4),
+        "b3_kv_attend_workspace": (ctypes.c_int64, [c_p] * 3),
+        "b3_kv_attend": (c_i, [c_p] * 4 + [ctypes.c_int64, c_p]),
+        "b3_sample": (c_i, [c_p] * 2),
         "b3_bark_ans_cdf": (c_i, [c_p, c_i, c_p]),
         "b3_bark_ans_decode": (c_i, [c_p, c_i, c_p, ctypes.c_int64, ctypes.c_int64, c_p]),
         "b3_bark_decode_levels2": (c_i, [c_p, ctypes.c_int64, c_p, ctypes.c_int64, c_i, c_i, c_i, c_p]),
@@ -411,3 +416,13 @@ def frames_for_seconds(seconds: float) -> int:
     for _ in range(3):
         v = (v - 1) // 2 + 1
     return v
+
+
+def __getattr__(name):
+    """KvCache and sample live in textgen.py, imported when first asked for."""
+    if name in ("KvCache", "sample"):
+        from . import textgen
+
+        globals()["KvCache"], globals()["sample"] = textgen.KvCache, textgen.sample
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

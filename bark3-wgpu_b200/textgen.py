@@ -1,0 +1,291 @@
+"""Text generation beside the encoder: a paged 8-bit cache of keys and values,
+the attention that reads it, and the choice of the next token.
+
+    cache = KvCache(pages, kv_heads, head_dim)
+    q = cache.append(q, k, v, cu_q, kv_lens, page_table, q_norm=..., k_norm=..., cos=..., sin=...)
+    out = cache.attend(q, cu_q, kv_lens, page_table, max_q=1)
+    ids, logprob = sample(logits, uniform, temperature=..., top_k=..., top_p=..., min_p=...)
+
+Everything is a torch tensor on one GPU.  The calls enqueue their work on
+torch's current stream of that GPU and return; they can be captured in a CUDA
+graph.  What they compute is written down at b3_kv_cache, b3_kv_append,
+b3_kv_attend and b3_sample in include/bark3_b200.h; a bad argument raises
+B3Error(B3_EINVAL), lengths or page numbers that only the GPU sees are reported
+by KvCache.check().
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import B3_EINVAL, B3_ETIMEOUT, DTYPE_BF16, DTYPE_F16, DTYPE_F32, B3Error, check, lib
+
+_P, _I32, _I64, _F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+
+KV_BAD_LENGTH, KV_BAD_PAGE, KV_BAD_POSITION, KV_TIMEOUT = 1, 2, 4, 8
+SAMPLE_MAX_VOCAB = 262144
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("status", _P), ("pages", _I32),
+                ("kv_heads", _I32), ("page_tokens", _I32), ("head_dim", _I32)]
+
+
+class _Batch(ctypes.Structure):
+    _fields_ = [("cu_q", _P), ("kv_lens", _P), ("page_table", _P), ("table_stride", _I64), ("table_width", _I32),
+                ("n_seq", _I32), ("tokens", _I32)]
+
+
+class _Append(ctypes.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_out", _P), ("q_token_stride", _I64), ("q_head_stride", _I64),
+                ("k_token_stride", _I64), ("k_head_stride", _I64), ("v_token_stride", _I64), ("v_head_stride", _I64),
+                ("q_norm", _P), ("k_norm", _P), ("cos", _P), ("sin", _P), ("positions", _P), ("eps", _F32),
+                ("dtype", _I32), ("out_dtype", _I32), ("q_heads", _I32), ("rot_dim", _I32), ("rot_rows", _I32),
+                ("interleaved", _I32)]
+
+
+class _Attend(ctypes.Structure):
+    _fields_ = [("q", _P), ("out", _P), ("lse", _P), ("q_token_stride", _I64), ("q_head_stride", _I64),
+                ("scale", _F32), ("dtype", _I32), ("q_heads", _I32), ("max_q", _I32), ("causal", _I32),
+                ("window", _I32)]
+
+
+class _Sample(ctypes.Structure):
+    _fields_ = [("logits", _P), ("uniform", _P), ("temperature", _P), ("top_k", _P), ("top_p", _P), ("min_p", _P),
+                ("ids", _P), ("logprob", _P), ("row_stride", _I64), ("dtype", _I32), ("rows", _I32), ("vocab", _I32)]
+
+
+_torch = None
+_DTYPES: dict = {}
+
+
+def _torch_module():
+    global _torch
+    if _torch is None:
+        import torch
+
+        _torch = torch
+        _DTYPES.update({torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16})
+    return _torch
+
+
+def _fail(msg: str):
+    raise B3Error(B3_EINVAL, msg)
+
+
+def _stream(index: int) -> int:
+    """torch's current stream on the GPU, as a cudaStream_t."""
+    return _torch.cuda.current_stream(index).cuda_stream
+
+
+class _On:
+    """Makes `device` current for a call when another one is."""
+
+    def __init__(self, index: int):
+        self.index, self.before = index, None
+
+    def __enter__(self):
+        now = _torch.cuda.current_device()
+        if now != self.index:
+            self.before = now
+            _torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before is not None:
+            _torch.cuda.set_device(self.before)
+
+
+def _vector(t, name, dtype, n, device):
+    """Address of a contiguous (n,) tensor, None where there is none."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.shape != (n,) or t.device != device or not t.is_contiguous():
+        _fail(f"{name} must be a contiguous {dtype} tensor of {n} on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+class KvCache:
+    """Keys and values of many sequences in 8 bits, in pages of `page_tokens`
+    tokens with a scale for each page and key head.
+
+    k, v               (pages, kv_heads, page_tokens, head_dim) float8_e4m3fn
+    k_scale, v_scale   (pages, kv_heads) float32, powers of two
+
+    Which pages a sequence has is the caller's page table: (n_seq, width)
+    int32, entry j of row i the page of tokens [j * page_tokens,
+    (j + 1) * page_tokens) of sequence i; entries past its last token are
+    never read.  Calls on one cache are made by one thread at a time."""
+
+    def __init__(self, pages: int, kv_heads: int, head_dim: int, page_tokens: int = 64, device: int = 0):
+        torch = _torch_module()
+        dev = torch.device("cuda", device)
+        shape = (pages, kv_heads, page_tokens, head_dim)
+        if min(shape) <= 0:
+            _fail(f"cache shape {shape}")
+        raw = [torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2)]
+        scales = [torch.ones(shape[:2], dtype=torch.float32, device=dev) for _ in range(2)]
+        self._hold(*raw, *scales)
+
+    @classmethod
+    def over(cls, k, v, k_scale, v_scale) -> "KvCache":
+        """A cache over the caller's own tensors."""
+        _torch_module()
+        self = cls.__new__(cls)
+        self._hold(k, v, k_scale, v_scale)
+        return self
+
+    def _hold(self, k, v, k_scale, v_scale) -> None:
+        torch = _torch
+        if k.dim() != 4 or not k.is_cuda:
+            _fail("k must be a (pages, kv_heads, page_tokens, head_dim) tensor on a GPU")
+        for t, name, dtype, shape in ((k, "k", torch.float8_e4m3fn, k.shape), (v, "v", torch.float8_e4m3fn, k.shape),
+                                      (k_scale, "k_scale", torch.float32, k.shape[:2]),
+                                      (v_scale, "v_scale", torch.float32, k.shape[:2])):
+            if t.dtype is not dtype or t.shape != shape or t.device != k.device or not t.is_contiguous():
+                _fail(f"{name} must be a contiguous {dtype} tensor of {tuple(shape)} on {k.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
+        self.device = k.device
+        self._status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._L = lib()
+        self._c = _Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self._status.data_ptr(),
+                         self.pages, self.kv_heads, self.page_tokens, self.head_dim)
+        self._b, self._app, self._att = _Batch(), _Append(), _Attend()
+        self._refs = [ctypes.byref(x) for x in (self._c, self._b, self._app, self._att)]
+
+    def check(self) -> None:
+        """Waits for the GPU and raises for what the calls since the last
+        check met that only the GPU could see."""
+        bits = int(self._status.item())
+        if not bits:
+            return
+        self._status.zero_()
+        if bits & KV_TIMEOUT:
+            raise B3Error(B3_ETIMEOUT, "a bounded wait inside the attention ran out")
+        what = [s for bit, s in ((KV_BAD_LENGTH, "cu_q or kv_lens out of range"),
+                                 (KV_BAD_PAGE, "a page number outside the cache"),
+                                 (KV_BAD_POSITION, "a position outside the cos / sin table")) if bits & bit]
+        _fail(", ".join(what))
+
+    def _batch(self, tokens, cu_q, kv_lens, page_table) -> None:
+        torch, b = _torch, self._b
+        n = kv_lens.shape[0]
+        b.cu_q = _vector(cu_q, "cu_q", torch.int32, n + 1, self.device)
+        b.kv_lens = _vector(kv_lens, "kv_lens", torch.int32, n, self.device)
+        if (page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != n
+                or page_table.device != self.device or page_table.stride(1) != 1):
+            _fail(f"page_table must be a ({n}, width) int32 tensor on {self.device} with adjacent entries")
+        b.page_table = page_table.data_ptr()
+        b.table_width = page_table.shape[1]
+        b.table_stride = max(page_table.stride(0), b.table_width)
+        b.n_seq, b.tokens = n, tokens
+
+    def _rows(self, t, name, tokens, dtype) -> tuple:
+        if (t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != self.head_dim or t.stride(2) != 1
+                or t.dtype is not dtype or t.device != self.device):
+            _fail(f"{name} must be ({tokens}, heads, {self.head_dim}) {dtype} on {self.device} with adjacent channels, "
+                  f"got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
+        return t.data_ptr(), t.stride(0), t.stride(1)
+
+    def _out(self, out, shape, dtype):
+        if out is None:
+            return _torch.empty(shape, dtype=dtype, device=self.device)
+        if out.shape != shape or out.dtype is not dtype or out.device != self.device or not out.is_contiguous():
+            _fail(f"out must be a contiguous {dtype} tensor of {tuple(shape)} on {self.device}")
+        return out
+
+    def append(self, q, k, v, cu_q, kv_lens, page_table, *, q_norm=None, k_norm=None, eps: float = 1e-6, cos=None,
+               sin=None, interleaved: bool = False, positions=None, out=None):
+        """Norms and rotates the new tokens' q (tokens, q_heads, head_dim) and
+        k (tokens, kv_heads, head_dim), stores k and v in the cache and returns
+        the queries, ready for attend(): in q's own type, or float16 for
+        float32 input.  kv_lens counts the new tokens already.  q, k and v may
+        be views of one projection's output."""
+        torch = _torch
+        tokens, dtype = q.shape[0], q.dtype
+        if dtype not in _DTYPES:
+            _fail(f"q must be float32, float16 or bfloat16, got {dtype}")
+        a = self._app
+        a.q, a.q_token_stride, a.q_head_stride = self._rows(q, "q", tokens, dtype)
+        a.k, a.k_token_stride, a.k_head_stride = self._rows(k, "k", tokens, dtype)
+        a.v, a.v_token_stride, a.v_head_stride = self._rows(v, "v", tokens, dtype)
+        if k.shape[1] != self.kv_heads or v.shape[1] != self.kv_heads:
+            _fail(f"k and v must have {self.kv_heads} heads")
+        self._batch(tokens, cu_q, kv_lens, page_table)
+        out_dtype = torch.float16 if dtype is torch.float32 else dtype
+        out = self._out(out, q.shape, out_dtype)
+        a.q_out, a.dtype, a.out_dtype, a.q_heads = out.data_ptr(), _DTYPES[dtype], _DTYPES[out_dtype], q.shape[1]
+        a.q_norm = _vector(q_norm, "q_norm", torch.float32, self.head_dim, self.device)
+        a.k_norm = _vector(k_norm, "k_norm", torch.float32, self.head_dim, self.device)
+        a.eps, a.interleaved = eps, interleaved
+        a.positions = _vector(positions, "positions", torch.int32, tokens, self.device)
+        if (cos is None) != (sin is None):
+            _fail("cos and sin come together")
+        if cos is None:
+            a.cos = a.sin = None
+        else:
+            for t, name in ((cos, "cos"), (sin, "sin")):
+                if t.dtype is not torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.device != self.device or not t.is_contiguous():
+                    _fail(f"{name} must be a contiguous float32 (positions, rot_dim / 2) tensor on {self.device}")
+            a.cos, a.sin, a.rot_rows, a.rot_dim = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
+        c, b, app, _ = self._refs
+        with _On(self.device.index):
+            check(self._L.b3_kv_append(c, b, app, _stream(self.device.index)))
+        return out
+
+    def attend(self, q, cu_q, kv_lens, page_table, *, max_q: int, scale: float | None = None, causal: bool = True,
+               window: int = 0, out=None, return_lse: bool = False):
+        """Attention of the new tokens' queries (tokens, q_heads, head_dim),
+        float16 or bfloat16, over the cached keys and values of their
+        sequences.  max_q: an upper bound of any sequence's new tokens.
+        scale: 1 / sqrt(head_dim) by default.  Returns out in q's type, with
+        return_lse also the (tokens, q_heads) float32 log-sum-exp."""
+        torch = _torch
+        tokens, dtype = q.shape[0], q.dtype
+        if dtype is not torch.float16 and dtype is not torch.bfloat16:
+            _fail(f"q must be float16 or bfloat16, got {dtype}")
+        a = self._att
+        a.q, a.q_token_stride, a.q_head_stride = self._rows(q, "q", tokens, dtype)
+        self._batch(tokens, cu_q, kv_lens, page_table)
+        out = self._out(out, q.shape, dtype)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) if return_lse else None
+        a.out, a.lse = out.data_ptr(), lse.data_ptr() if return_lse else None
+        a.scale = self.head_dim ** -0.5 if scale is None else scale
+        a.dtype, a.q_heads, a.max_q, a.causal, a.window = _DTYPES[dtype], q.shape[1], max_q, causal, window
+        c, b, _, att = self._refs
+        with _On(self.device.index):
+            need = self._L.b3_kv_attend_workspace(c, b, att)
+            if need < 0:
+                check(need)
+            # from torch's allocator on the current stream: calls on other streams get other memory
+            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            check(self._L.b3_kv_attend(c, b, att, work.data_ptr() if need else None, need, _stream(self.device.index)))
+        return (out, lse) if return_lse else out
+
+    def values(self, page: int):
+        """The (kv_heads, page_tokens, head_dim) float32 keys and values that a page stands for."""
+        return (self.k[page].float() * self.k_scale[page][:, None, None],
+                self.v[page].float() * self.v_scale[page][:, None, None])
+
+
+def sample(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=None):
+    """The next token of every row of logits (rows, vocab), float32, float16 or
+    bfloat16: (ids int32, logprob float32), each (rows,).  uniform and the
+    settings are (rows,) tensors on the logits' GPU (top_k int32, the others
+    float32); None leaves a setting off (temperature: 1)."""
+    torch = _torch_module()
+    if logits.dim() != 2 or not logits.is_cuda or logits.stride(1) != 1 or logits.dtype not in _DTYPES:
+        _fail("logits must be a (rows, vocab) float32, float16 or bfloat16 tensor on a GPU with adjacent columns")
+    rows, vocab = logits.shape
+    dev = logits.device
+    if uniform is None:
+        _fail("uniform is missing")
+    ids = torch.empty(rows, dtype=torch.int32, device=dev)
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    a = _Sample(logits.data_ptr(), _vector(uniform, "uniform", torch.float32, rows, dev),
+                _vector(temperature, "temperature", torch.float32, rows, dev),
+                _vector(top_k, "top_k", torch.int32, rows, dev), _vector(top_p, "top_p", torch.float32, rows, dev),
+                _vector(min_p, "min_p", torch.float32, rows, dev), ids.data_ptr(), logprob.data_ptr(),
+                max(logits.stride(0), vocab), _DTYPES[logits.dtype], rows, vocab)
+    with _On(dev.index):
+        check(lib().b3_sample(ctypes.byref(a), _stream(dev.index)))
+    return ids, logprob

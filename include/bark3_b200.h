@@ -246,6 +246,148 @@ int b3_linear_lut4_noalloc(const float* a, const uint8_t* codes, const uint16_t*
  * x is [t][1024]. */
 int b3_attn_conv(b3_ctx* ctx, int layer, float* x, int t, unsigned flags);
 
+/* ─────────────────────────── text generation ───────────────────────────
+ * One decode step of an attention decoder that reads the encoder's frames (or
+ * text) as its prompt: b3_kv_append, b3_kv_attend, b3_sample.  No counterpart
+ * in the reference, whose decoder is the greedy TDT.
+ *
+ * These calls need no context.  All data pointers are device pointers of the
+ * current device, the structs themselves are host memory and are read during
+ * the call; the work is enqueued on `stream` (a cudaStream_t, NULL = legacy
+ * default stream), nothing is allocated and nothing waits, so the calls can
+ * be captured in a CUDA graph.  Arguments that the host can see are checked
+ * before anything is launched (B3_EINVAL).  Lengths and page numbers live on
+ * the device; a kernel that meets one out of range skips that access and sets
+ * a B3_KV_BAD_* bit in the cache's status word.
+ *
+ * The cache holds 8-bit floats (e4m3: 4 exponent and 3 mantissa bits, largest
+ * 448) and a scale for each page and head that is a power of two:
+ *   k, v              [pages][kv_heads][page_tokens][head_dim] e4m3
+ *   k_scale, v_scale  [pages][kv_heads] f32, 2^e with e in [-40, 40]
+ * value = code * scale.  e is the least with every finite value of the page
+ * at most 448 * 2^e in magnitude; larger magnitudes (at e = 40) and
+ * infinities are held as +-448 * 2^e, NaN stays NaN.  While a page holds
+ * tokens its scale only grows; codes held then are divided by the same power
+ * of two, which is exact except where the code falls below e4m3's normal
+ * range (2^-6).  The first token of a page forgets the page's old scale. */
+typedef struct b3_kv_cache {
+    uint8_t* k;
+    uint8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int32_t* status;      /* one word, B3_KV_BAD_* bits are or-ed into it; may be NULL */
+    int32_t pages;        /* pages * kv_heads * page_tokens < 2^31 */
+    int32_t kv_heads;
+    int32_t page_tokens;  /* 16, 32, 64 or 128 */
+    int32_t head_dim;     /* 64 or 128 */
+} b3_kv_cache;
+
+#define B3_KV_BAD_LENGTH 1    /* cu_q or kv_lens out of range */
+#define B3_KV_BAD_PAGE 2      /* a page number outside the cache */
+#define B3_KV_BAD_POSITION 4  /* a position outside the cos / sin table */
+#define B3_KV_TIMEOUT 8       /* a bounded wait inside the attention ran out */
+
+/* The sequences of one call.  Sequence i has the new tokens (rows of q, k, v)
+ * cu_q[i] .. cu_q[i+1], which are the last of its kv_lens[i] tokens; token j
+ * of it lives in slot j % page_tokens of page page_table[i][j / page_tokens].
+ * Table entries past the last token are never read.  A sequence may have no
+ * new tokens, or (attention only) no tokens at all. */
+typedef struct b3_kv_batch {
+    const int32_t* cu_q;        /* [n_seq + 1], cu_q[0] = 0, cu_q[n_seq] = tokens */
+    const int32_t* kv_lens;     /* [n_seq], the new tokens included */
+    const int32_t* page_table;  /* [n_seq][table_stride], table_width entries in use */
+    int64_t table_stride;
+    int32_t table_width;
+    int32_t n_seq;
+    int32_t tokens;
+} b3_kv_batch;
+
+/* New queries, keys and values into the step: for each head of q and k an
+ * optional RMS norm, x / sqrt(mean(x^2) + eps) * weight, then the rotation of
+ * the first rot_dim channels by the token's position; the queries leave as
+ * q_out, keys and values (v untouched) go into the cache.  Arithmetic in f32;
+ * the one rounding of q_out and of each code comes last.  A row's channels are
+ * contiguous; token and head strides (in elements) are free. */
+typedef struct b3_kv_append_args {
+    const void* q;   /* [tokens][q_heads][head_dim], dtype */
+    const void* k;   /* [tokens][kv_heads][head_dim], dtype */
+    const void* v;   /* same */
+    void* q_out;     /* [tokens][q_heads][head_dim], out_dtype (f16 or bf16), contiguous */
+    int64_t q_token_stride, q_head_stride;
+    int64_t k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride;
+    const float* q_norm;      /* [head_dim] or NULL: no norm */
+    const float* k_norm;      /* [head_dim] or NULL */
+    const float* cos;         /* [rot_rows][rot_dim / 2] or NULL: no rotation */
+    const float* sin;         /* same */
+    const int32_t* positions; /* [tokens], or NULL: a token's index in its sequence */
+    float eps;
+    int32_t dtype;            /* B3_DTYPE_F32, F16 or BF16 */
+    int32_t out_dtype;        /* B3_DTYPE_F16 or BF16 */
+    int32_t q_heads;          /* a multiple of kv_heads */
+    int32_t rot_dim;          /* a multiple of 16, at most head_dim */
+    int32_t rot_rows;
+    int32_t interleaved;      /* 0: channels i and i + rot_dim/2 turn together, 1: 2i and 2i + 1 */
+} b3_kv_append_args;
+int b3_kv_append(const b3_kv_cache* cache, const b3_kv_batch* batch, const b3_kv_append_args* args, void* stream);
+
+/* Attention of the new tokens' queries over the cached ones:
+ *   out = softmax_j(scale * q . k_j) v_j over the keys j that the query sees,
+ * query head h with key head h / (q_heads / kv_heads).  With `causal` the
+ * token at index p of its sequence sees keys 0 .. p, and with window > 0 of
+ * those only the last `window`; otherwise every query sees all of its
+ * sequence.  A query that sees no key gives zeros and lse = -inf.  lse is the
+ * natural logarithm of the sum of exponentials.  Scores, softmax and sums are
+ * f32; the products' operands are the e4m3 codes and 16-bit queries, both
+ * exact, and probabilities rounded to f16.
+ * `max_q` is an upper bound of the new tokens of any one sequence.
+ * `workspace` (16-byte aligned, b3_kv_attend_workspace bytes) is scratch of
+ * this call alone: calls that may overlap need one each. */
+typedef struct b3_kv_attend_args {
+    const void* q;     /* [tokens][q_heads][head_dim], dtype */
+    void* out;         /* same shape and dtype, contiguous */
+    float* lse;        /* [tokens][q_heads] or NULL */
+    int64_t q_token_stride, q_head_stride;
+    float scale;
+    int32_t dtype;     /* B3_DTYPE_F16 or BF16 */
+    int32_t q_heads;   /* a multiple of kv_heads */
+    int32_t max_q;
+    int32_t causal;
+    int32_t window;    /* 0: none; needs causal */
+} b3_kv_attend_args;
+int64_t b3_kv_attend_workspace(const b3_kv_cache* cache, const b3_kv_batch* batch, const b3_kv_attend_args* args);
+int b3_kv_attend(const b3_kv_cache* cache, const b3_kv_batch* batch, const b3_kv_attend_args* args, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
+/* The next token of every row of logits.  With m the row's largest logit,
+ * token i weighs w_i = exp((l_i - m) / temperature) (f32, held as a whole
+ * number of 2^-31, so that sums are exact and the answer does not depend on
+ * their order; -inf and NaN logits weigh nothing).  In the order of falling
+ * logits, ties by rising index, top_k keeps the first top_k tokens, top_p of
+ * those the shortest beginning whose weight reaches top_p of theirs, and
+ * min_p drops what weighs less than min_p; the largest always stays (unless
+ * min_p > 1).  The answer is the first kept token, by index, at which the
+ * running sum of kept weights exceeds uniform times their total.
+ * temperature <= 0 takes the largest logit, the lowest index of equals.  A
+ * row without a finite or +inf logit, or with nothing kept, gives id -1 and
+ * logprob NaN.  logprob is the logarithm of the token's weight over the total. */
+typedef struct b3_sample_args {
+    const void* logits;        /* [rows][vocab], dtype; rows row_stride elements apart */
+    const float* uniform;      /* [rows] in [0, 1) */
+    const float* temperature;  /* [rows] or NULL: 1 */
+    const int32_t* top_k;      /* [rows] or NULL; <= 0: off */
+    const float* top_p;        /* [rows] or NULL; >= 1: off */
+    const float* min_p;        /* [rows] or NULL; <= 0: off */
+    int32_t* ids;              /* [rows] */
+    float* logprob;            /* [rows] or NULL */
+    int64_t row_stride;
+    int32_t dtype;             /* B3_DTYPE_F32, F16 or BF16 */
+    int32_t rows;
+    int32_t vocab;             /* at most B3_SAMPLE_MAX_VOCAB */
+} b3_sample_args;
+#define B3_SAMPLE_MAX_VOCAB 262144
+int b3_sample(const b3_sample_args* args, void* stream);
+
 /* ─────────────────────── .bark container streams ───────────────────────
  * Host-only entropy decoding of the `model.bark` weight container (no GPU
  * work; callable without a device).  The container's JSON index, LZMA fields
