@@ -3,18 +3,12 @@
 //   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale q_i . k_j - m_i)
 // with k_j = code * 2^e of the page, in one pass over the keys with a running
 // maximum m and sum.  One warp for each (token, query head).
-#include "kv_cache.cuh"
+#include "kv_attend.cuh"
 
 namespace b3 {
 namespace {
 
 constexpr int kThreads = 128;
-
-struct AttendParams {
-    b3_kv_cache c;
-    b3_kv_batch b;
-    b3_kv_attend_args a;
-};
 
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kThreads) k_kv_attend_row(const __grid_constant__ AttendParams p) {
@@ -103,9 +97,15 @@ int launch(const AttendParams& p, cudaStream_t st) {
 
 using namespace b3;
 
+static bool few_rows(const b3_kv_cache& c, const b3_kv_attend_args& a) {
+    return static_cast<int64_t>(a.max_q) * (a.q_heads / c.kv_heads) <= 16;
+}
+
 extern "C" int64_t b3_kv_attend_workspace(const b3_kv_cache* cache, const b3_kv_batch* batch,
                                           const b3_kv_attend_args* args) {
-    return check(cache, batch, args);
+    if (int rc = check(cache, batch, args)) return rc;
+    const AttendParams p{*cache, *batch, *args};
+    return few_rows(*cache, *args) ? attend_rows_workspace(p) : 0;
 }
 
 extern "C" int b3_kv_attend(const b3_kv_cache* cache, const b3_kv_batch* batch, const b3_kv_attend_args* args,
@@ -114,9 +114,14 @@ extern "C" int b3_kv_attend(const b3_kv_cache* cache, const b3_kv_batch* batch, 
     if (batch->tokens == 0) return 0;
     if (!args->q || !args->out) return set_error(B3_EINVAL, "null q or out");
     if (reinterpret_cast<uintptr_t>(args->out) & 15) return set_error(B3_EINVAL, "out must be 16-byte aligned");
-    (void)workspace;
-    (void)workspace_bytes;
-    AttendParams p{*cache, *batch, *args};
+    const AttendParams p{*cache, *batch, *args};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (few_rows(*cache, *args)) {
+        const int64_t need = attend_rows_workspace(p);
+        if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
+            return set_error(B3_EINVAL, "workspace of %lld bytes, 16-byte aligned, is needed (got %lld)",
+                             static_cast<long long>(need), static_cast<long long>(workspace_bytes));
+        return launch_attend_rows(p, workspace, st);
+    }
     return args->dtype == B3_DTYPE_F16 ? launch<__half>(p, st) : launch<__nv_bfloat16>(p, st);
 }
