@@ -16,6 +16,8 @@ by KvCache.check().
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 
 from . import B3_EINVAL, B3_ETIMEOUT, DTYPE_BF16, DTYPE_F16, DTYPE_F32, B3Error, check, lib
 
@@ -54,6 +56,19 @@ class _Sample(ctypes.Structure):
                 ("ids", _P), ("logprob", _P), ("row_stride", _I64), ("dtype", _I32), ("rows", _I32), ("vocab", _I32)]
 
 
+class _Args:
+    """Memory of one argument struct, filled by a single pack: `set(...)`
+    takes the fields in order, 0 for a NULL pointer, and `at` is its address."""
+
+    _CODES = {_P: "P", _I32: "i", _I64: "q", _F32: "f"}
+
+    def __init__(self, layout):
+        self._buf = ctypes.create_string_buffer(ctypes.sizeof(layout))
+        pack = struct.Struct("@" + "".join(self._CODES[t] for _, t in layout._fields_))
+        self.set = functools.partial(pack.pack_into, self._buf, 0)
+        self.at = ctypes.addressof(self._buf)
+
+
 _torch = None
 _DTYPES: dict = {}
 
@@ -72,34 +87,26 @@ def _fail(msg: str):
     raise B3Error(B3_EINVAL, msg)
 
 
-def _stream(index: int) -> int:
-    """torch's current stream on the GPU, as a cudaStream_t."""
-    return _torch.cuda.current_stream(index).cuda_stream
+def _launch(fn, index: int, *args) -> None:
+    """fn(*args, stream) on torch's current stream of GPU `index`, with that GPU current."""
+    torch = _torch
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        check(rc)
 
 
-class _On:
-    """Makes `device` current for a call when another one is."""
-
-    def __init__(self, index: int):
-        self.index, self.before = index, None
-
-    def __enter__(self):
-        now = _torch.cuda.current_device()
-        if now != self.index:
-            self.before = now
-            _torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before is not None:
-            _torch.cuda.set_device(self.before)
-
-
-def _vector(t, name, dtype, n, device):
-    """Address of a contiguous (n,) tensor, None where there is none."""
+def _vector(t, name, dtype, n, index):
+    """Address of a contiguous (n,) tensor on GPU `index`, 0 where there is none."""
     if t is None:
-        return None
-    if t.dtype is not dtype or t.shape != (n,) or t.device != device or not t.is_contiguous():
-        _fail(f"{name} must be a contiguous {dtype} tensor of {n} on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        return 0
+    if t.dtype is not dtype or t.dim() != 1 or t.size(0) != n or t.get_device() != index or not t.is_contiguous():
+        _fail(f"{name} must be a contiguous {dtype} tensor of {n} on cuda:{index}, "
+              f"got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
@@ -146,11 +153,12 @@ class KvCache:
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
         self.device = k.device
         self._status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._index = k.get_device()
         self._L = lib()
-        self._c = _Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self._status.data_ptr(),
-                         self.pages, self.kv_heads, self.page_tokens, self.head_dim)
-        self._b, self._app, self._att = _Batch(), _Append(), _Attend()
-        self._refs = [ctypes.byref(x) for x in (self._c, self._b, self._app, self._att)]
+        self._c, self._b, self._app, self._att = (_Args(x) for x in (_Cache, _Batch, _Append, _Attend))
+        self._c.set(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self._status.data_ptr(),
+                    self.pages, self.kv_heads, self.page_tokens, self.head_dim)
+        self._work: dict = {}   # workspace bytes by what they depend on
 
     def check(self) -> None:
         """Waits for the GPU and raises for what the calls since the last
@@ -166,31 +174,30 @@ class KvCache:
                                  (KV_BAD_POSITION, "a position outside the cos / sin table")) if bits & bit]
         _fail(", ".join(what))
 
-    def _batch(self, tokens, cu_q, kv_lens, page_table) -> None:
-        torch, b = _torch, self._b
-        n = kv_lens.shape[0]
-        b.cu_q = _vector(cu_q, "cu_q", torch.int32, n + 1, self.device)
-        b.kv_lens = _vector(kv_lens, "kv_lens", torch.int32, n, self.device)
-        if (page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != n
-                or page_table.device != self.device or page_table.stride(1) != 1):
+    def _batch(self, tokens, cu_q, kv_lens, page_table) -> int:
+        i32, index = _torch.int32, self._index
+        n = kv_lens.size(0) if kv_lens.dim() == 1 else -1
+        cu, lens = _vector(cu_q, "cu_q", i32, n + 1, index), _vector(kv_lens, "kv_lens", i32, n, index)
+        if (page_table.dtype is not i32 or page_table.dim() != 2 or page_table.size(0) != n
+                or page_table.get_device() != index or page_table.stride(1) != 1):
             _fail(f"page_table must be a ({n}, width) int32 tensor on {self.device} with adjacent entries")
-        b.page_table = page_table.data_ptr()
-        b.table_width = page_table.shape[1]
-        b.table_stride = max(page_table.stride(0), b.table_width)
-        b.n_seq, b.tokens = n, tokens
+        width = page_table.size(1)
+        self._b.set(cu, lens, page_table.data_ptr(), max(page_table.stride(0), width), width, n, tokens)
+        return n
 
-    def _rows(self, t, name, tokens, dtype) -> tuple:
-        if (t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != self.head_dim or t.stride(2) != 1
-                or t.dtype is not dtype or t.device != self.device):
-            _fail(f"{name} must be ({tokens}, heads, {self.head_dim}) {dtype} on {self.device} with adjacent channels, "
-                  f"got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
-        return t.data_ptr(), t.stride(0), t.stride(1)
+    def _rows(self, t, name, tokens, heads, dtype):
+        """Address of new rows (tokens, heads, head_dim), heads of any number where `heads` is None."""
+        if (t.dtype is not dtype or t.dim() != 3 or t.size(0) != tokens or t.size(2) != self.head_dim
+                or (heads is not None and t.size(1) != heads) or t.stride(2) != 1 or t.get_device() != self._index):
+            _fail(f"{name} must be ({tokens}, {heads or 'heads'}, {self.head_dim}) {dtype} on {self.device} with "
+                  f"adjacent channels, got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
+        return t.data_ptr()
 
-    def _out(self, out, shape, dtype):
+    def _out(self, out, like, dtype):
         if out is None:
-            return _torch.empty(shape, dtype=dtype, device=self.device)
-        if out.shape != shape or out.dtype is not dtype or out.device != self.device or not out.is_contiguous():
-            _fail(f"out must be a contiguous {dtype} tensor of {tuple(shape)} on {self.device}")
+            return _torch.empty(like.shape, dtype=dtype, device=self.device)
+        if out.shape != like.shape or out.dtype is not dtype or out.get_device() != self._index or not out.is_contiguous():
+            _fail(f"out must be a contiguous {dtype} tensor of {tuple(like.shape)} on {self.device}")
         return out
 
     def append(self, q, k, v, cu_q, kv_lens, page_table, *, q_norm=None, k_norm=None, eps: float = 1e-6, cos=None,
@@ -200,36 +207,31 @@ class KvCache:
         the queries, ready for attend(): in q's own type, or float16 for
         float32 input.  kv_lens counts the new tokens already.  q, k and v may
         be views of one projection's output."""
-        torch = _torch
-        tokens, dtype = q.shape[0], q.dtype
-        if dtype not in _DTYPES:
+        torch, index, f32 = _torch, self._index, _torch.float32
+        tokens, dtype = q.size(0), q.dtype
+        code = _DTYPES.get(dtype)
+        if code is None:
             _fail(f"q must be float32, float16 or bfloat16, got {dtype}")
-        a = self._app
-        a.q, a.q_token_stride, a.q_head_stride = self._rows(q, "q", tokens, dtype)
-        a.k, a.k_token_stride, a.k_head_stride = self._rows(k, "k", tokens, dtype)
-        a.v, a.v_token_stride, a.v_head_stride = self._rows(v, "v", tokens, dtype)
-        if k.shape[1] != self.kv_heads or v.shape[1] != self.kv_heads:
-            _fail(f"k and v must have {self.kv_heads} heads")
+        at_q = self._rows(q, "q", tokens, None, dtype)
+        at_k = self._rows(k, "k", tokens, self.kv_heads, dtype)
+        at_v = self._rows(v, "v", tokens, self.kv_heads, dtype)
         self._batch(tokens, cu_q, kv_lens, page_table)
-        out_dtype = torch.float16 if dtype is torch.float32 else dtype
-        out = self._out(out, q.shape, out_dtype)
-        a.q_out, a.dtype, a.out_dtype, a.q_heads = out.data_ptr(), _DTYPES[dtype], _DTYPES[out_dtype], q.shape[1]
-        a.q_norm = _vector(q_norm, "q_norm", torch.float32, self.head_dim, self.device)
-        a.k_norm = _vector(k_norm, "k_norm", torch.float32, self.head_dim, self.device)
-        a.eps, a.interleaved = eps, interleaved
-        a.positions = _vector(positions, "positions", torch.int32, tokens, self.device)
+        out_code = DTYPE_F16 if code == DTYPE_F32 else code
+        out = self._out(out, q, torch.float16 if code == DTYPE_F32 else dtype)
         if (cos is None) != (sin is None):
             _fail("cos and sin come together")
-        if cos is None:
-            a.cos = a.sin = None
-        else:
+        at_cos = at_sin = rot_dim = rot_rows = 0
+        if cos is not None:
             for t, name in ((cos, "cos"), (sin, "sin")):
-                if t.dtype is not torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.device != self.device or not t.is_contiguous():
+                if t.dtype is not f32 or t.dim() != 2 or t.shape != cos.shape or t.get_device() != index or not t.is_contiguous():
                     _fail(f"{name} must be a contiguous float32 (positions, rot_dim / 2) tensor on {self.device}")
-            a.cos, a.sin, a.rot_rows, a.rot_dim = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
-        c, b, app, _ = self._refs
-        with _On(self.device.index):
-            check(self._L.b3_kv_append(c, b, app, _stream(self.device.index)))
+            at_cos, at_sin, rot_rows, rot_dim = cos.data_ptr(), sin.data_ptr(), cos.size(0), 2 * cos.size(1)
+        self._app.set(at_q, at_k, at_v, out.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
+                      v.stride(1), _vector(q_norm, "q_norm", f32, self.head_dim, index),
+                      _vector(k_norm, "k_norm", f32, self.head_dim, index), at_cos, at_sin,
+                      _vector(positions, "positions", torch.int32, tokens, index), eps, code, out_code, q.size(1),
+                      rot_dim, rot_rows, interleaved)
+        _launch(self._L.b3_kv_append, index, self._c.at, self._b.at, self._app.at)
         return out
 
     def attend(self, q, cu_q, kv_lens, page_table, *, max_q: int, scale: float | None = None, causal: bool = True,
@@ -239,26 +241,29 @@ class KvCache:
         sequences.  max_q: an upper bound of any sequence's new tokens.
         scale: 1 / sqrt(head_dim) by default.  Returns out in q's type, with
         return_lse also the (tokens, q_heads) float32 log-sum-exp."""
-        torch = _torch
-        tokens, dtype = q.shape[0], q.dtype
+        torch, index = _torch, self._index
+        tokens, heads, dtype = q.size(0), q.size(1), q.dtype
         if dtype is not torch.float16 and dtype is not torch.bfloat16:
             _fail(f"q must be float16 or bfloat16, got {dtype}")
-        a = self._att
-        a.q, a.q_token_stride, a.q_head_stride = self._rows(q, "q", tokens, dtype)
-        self._batch(tokens, cu_q, kv_lens, page_table)
-        out = self._out(out, q.shape, dtype)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) if return_lse else None
-        a.out, a.lse = out.data_ptr(), lse.data_ptr() if return_lse else None
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
-        a.dtype, a.q_heads, a.max_q, a.causal, a.window = _DTYPES[dtype], q.shape[1], max_q, causal, window
-        c, b, _, att = self._refs
-        with _On(self.device.index):
-            need = self._L.b3_kv_attend_workspace(c, b, att)
+        at_q = self._rows(q, "q", tokens, None, dtype)
+        n = self._batch(tokens, cu_q, kv_lens, page_table)
+        out = self._out(out, q, dtype)
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) if return_lse else None
+        self._att.set(at_q, out.data_ptr(), lse.data_ptr() if return_lse else 0, q.stride(0), q.stride(1),
+                      self.head_dim ** -0.5 if scale is None else scale, _DTYPES[dtype], heads, max_q, causal, window)
+        key = (n, tokens, heads, max_q)
+        need = self._work.get(key)
+        if need is None:
+            with torch.cuda.device(index):
+                need = self._L.b3_kv_attend_workspace(self._c.at, self._b.at, self._att.at)
             if need < 0:
                 check(need)
-            # from torch's allocator on the current stream: calls on other streams get other memory
-            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            check(self._L.b3_kv_attend(c, b, att, work.data_ptr() if need else None, need, _stream(self.device.index)))
+            if len(self._work) >= 1024:
+                self._work.clear()
+            self._work[key] = need
+        # from torch's allocator on the current stream: calls on other streams get other memory
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        _launch(self._L.b3_kv_attend, index, self._c.at, self._b.at, self._att.at, work.data_ptr() if need else 0, need)
         return (out, lse) if return_lse else out
 
     def values(self, page: int):
@@ -279,13 +284,13 @@ def sample(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=N
     dev = logits.device
     if uniform is None:
         _fail("uniform is missing")
+    index, f32 = logits.get_device(), torch.float32
     ids = torch.empty(rows, dtype=torch.int32, device=dev)
-    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    a = _Sample(logits.data_ptr(), _vector(uniform, "uniform", torch.float32, rows, dev),
-                _vector(temperature, "temperature", torch.float32, rows, dev),
-                _vector(top_k, "top_k", torch.int32, rows, dev), _vector(top_p, "top_p", torch.float32, rows, dev),
-                _vector(min_p, "min_p", torch.float32, rows, dev), ids.data_ptr(), logprob.data_ptr(),
-                max(logits.stride(0), vocab), _DTYPES[logits.dtype], rows, vocab)
-    with _On(dev.index):
-        check(lib().b3_sample(ctypes.byref(a), _stream(dev.index)))
+    logprob = torch.empty(rows, dtype=f32, device=dev)
+    a = _Args(_Sample)
+    a.set(logits.data_ptr(), _vector(uniform, "uniform", f32, rows, index),
+          _vector(temperature, "temperature", f32, rows, index), _vector(top_k, "top_k", torch.int32, rows, index),
+          _vector(top_p, "top_p", f32, rows, index), _vector(min_p, "min_p", f32, rows, index), ids.data_ptr(),
+          logprob.data_ptr(), max(logits.stride(0), vocab), _DTYPES[logits.dtype], rows, vocab)
+    _launch(lib().b3_sample, index, a.at)
     return ids, logprob
