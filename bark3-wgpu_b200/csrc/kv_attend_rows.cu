@@ -13,19 +13,21 @@
 // that k_join adds up in run order (same bits every time).
 //
 // A step.  Each warp has its own ring of stages in shared memory, filled by
-// TMA boxes of a page's rows, lines of 128 bytes in the 128-byte swizzle.
-//   scores  S[rows, 8 keys] += Q[rows, 16 dims] K^T   mma m16n8k16, B = K codes
-//   output  O[rows, 8 dims] += P[rows, 16 keys] V     mma m16n8k16, B = V codes
-// The S tile's accumulator layout is P's operand layout, so probabilities never
-// leave registers.  Which 16 channels an MMA step takes and which output
-// channel a column stands for are free choices: a lane takes 16 consecutive
-// bytes of a K row as four steps' operands, and of a V row as the same column
-// of 16 tiles, so both come by 16-byte loads; a V operand pairs two keys, two
-// byte permutes for four channels.  Which key a score column stands for is
-// free as well (key_of_col): chosen so that both kinds of load touch every
-// bank once.  m16n8k16 on mma.sync suffices here: at 16 rows the products need
-// a third of its rate when memory is saturated, and tcgen05's 128-row tiles
-// would multiply zeros.
+// TMA boxes of a page's rows, lines of 128 bytes in the 128-byte swizzle.  Both
+// products are transposed, the codes being the MMA's 16-row operand, so a tile
+// of eight query rows wastes nothing (mma m16n8k16, f16 -> f32):
+//   S^T[16 keys, 8 rows] += K[16 keys, 16 channels] Q^T
+//   O^T[16 channels, 8 rows] += V^T[16 channels, 16 keys] P^T
+// P^T's operand layout is S^T's accumulator layout with each 8 x 8 block
+// transposed (movmatrix), so probabilities never leave registers.  Which 16
+// channels an MMA step takes and which channel an output row stands for are
+// free choices: a lane takes 16 consecutive bytes of a K row as four steps'
+// operands, and of a V row as the same row of 16 tiles' columns, so both come
+// by 16-byte loads; a V operand pairs two keys, two byte permutes for four
+// channels.  Which key a score row stands for is free as well (key_of_row):
+// chosen so that both kinds of load touch every bank once.  mma.sync suffices
+// here: at eight rows the products need a sixth of its rate when memory is
+// saturated, and tcgen05's 128-row tiles would hold one token's few rows.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,13 +38,16 @@ namespace b3 {
 namespace {
 
 constexpr int kStep = 32;           // keys
+constexpr int kTilesM = kStep / 16; // MMA tiles of 16 keys
 constexpr int kMaxSeqs = 1024;      // sequences a launch
 constexpr int kMinRun = 2;          // steps a run at least
 
-template <int DIM>
+template <int DIM, int ROWS>
 struct Cfg {
-    static constexpr int kWarps = 8;
-    static constexpr int kStages = DIM == 128 ? 3 : 6;
+    // eight rows leave registers for ten warps: 94 against 101 us for eight warps with three stages
+    // (ragged batch of 128); the ring takes what shared memory there is
+    static constexpr int kWarps = ROWS == 8 ? 10 : 8;
+    static constexpr int kStages = (ROWS == 8 ? 2 : 3) * 128 / DIM;
     static constexpr uint32_t kHalf = kStep * DIM;             // K (or V) bytes of a stage
     static constexpr uint32_t kStage = 2 * kHalf;
     static constexpr uint32_t kRing = kWarps * kStages * kStage;
@@ -58,18 +63,25 @@ struct RowsParams {
     float* part;           // [workers][2][rows][DIM] outputs, then [workers][2][rows][2] (m, l)
 };
 
-// Score column c (0..7) of a tile stands for this key of the tile's eight.
+// Score row c (0..7) of a tile's half stands for this key of the half's eight.
 template <int DIM>
-__device__ __forceinline__ int key_of_col(int c) {
+__device__ __forceinline__ int key_of_row(int c) {
     return DIM == 128 ? c ^ ((c & 1) << 2) : c ^ ((c >> 1) & 1);
 }
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
     asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {   // of an 8 x 8 block of 16-bit values over the warp
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 __device__ __forceinline__ uint32_t codes2(uint32_t two) {   // two e4m3 codes -> f16x2
@@ -159,10 +171,11 @@ __device__ __forceinline__ int64_t run_length(int64_t total, int workers) {
     return max(static_cast<int64_t>(kMinRun), (total + workers - 1) / workers);
 }
 
-template <typename T>
-__device__ __forceinline__ void store_row(const AttendParams& p, int token, int head, int d, const float* o, int n, float inv) {
+template <typename T, int N>
+__device__ __forceinline__ void store_row(const AttendParams& p, int token, int head, int d, const float (&o)[N], float inv) {
     T* out = static_cast<T*>(p.a.out) + (static_cast<int64_t>(token) * p.a.q_heads + head) * p.c.head_dim + d;
-    for (int i = 0; i < n; i += 8) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = o[i + j] * inv;
@@ -171,12 +184,12 @@ __device__ __forceinline__ void store_row(const AttendParams& p, int token, int 
 }
 
 template <typename T, int DIM, int ROWS>
-__global__ void __launch_bounds__(Cfg<DIM>::kWarps * 32, 1)
+__global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
     k_attend_rows(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const __grid_constant__ RowsParams r) {
-    using C = Cfg<DIM>;
-    constexpr int kTiles = DIM / 8;      // output tiles of 8 channels; also 2 x the MMA steps over the channels
-    constexpr int kHalves = ROWS / 8;    // 1: rows 8..15 of the MMA tile are empty
+    using C = Cfg<DIM, ROWS>;
+    constexpr int kSteps = DIM / 16;     // MMA steps over the channels; also output tiles of 16 channels
+    constexpr int kHalves = ROWS / 8;    // tiles of eight query rows
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     int* prefix = reinterpret_cast<int*>(smem + C::kPrefix);
@@ -215,33 +228,32 @@ __global__ void __launch_bounds__(Cfg<DIM>::kWarps * 32, 1)
         const int n_steps = key1 > key0 ? (key1 - key0 + kStep - 1) / kStep : 0;
         const int n_rows = sp.n * group;
 
-        // pages: lane i of a group of 32 holds page `page0 + i`, its number and scales
+        // pages: lane i holds the number and scales of page `page0 + i`, and the number of page `page0 + 32 + i`
         const int page_last = (key1 - 1) >> log_page;
         int page0 = key0 >> log_page;
-        auto load_pages = [&](int from, int& id, float& ks, float& vs) {
-            id = 0;
-            ks = vs = 1.f;
-            if (from + lane <= page_last) {
-                id = __ldg(p.b.page_table + seq * p.b.table_stride + from + lane);
+        auto load_id = [&](int pg) {
+            int id = 0;
+            if (pg <= page_last) {
+                id = __ldg(p.b.page_table + seq * p.b.table_stride + pg);
                 if (id < 0 || id >= p.c.pages) {
                     kv_flag(p.c.status, B3_KV_BAD_PAGE);
                     id = 0;
                 }
-                const int64_t slab = static_cast<int64_t>(id) * heads + it.head;
-                ks = __ldg(p.c.k_scale + slab);
-                vs = __ldg(p.c.v_scale + slab);
             }
+            return id;
         };
-        int id_a, id_b;
-        float ks_a, vs_a, ks_b, vs_b;
+        auto load_scale = [&](const float* scale, int id) { return __ldg(scale + static_cast<int64_t>(id) * heads + it.head); };
+        int id_a = 0, id_b = 0;
+        float ks_a = 1.f, vs_a = 1.f;
         if (n_steps) {
-            load_pages(page0, id_a, ks_a, vs_a);
-            load_pages(page0 + 32, id_b, ks_b, vs_b);
+            id_a = load_id(page0 + lane);
+            id_b = load_id(page0 + 32 + lane);
+            ks_a = load_scale(p.c.k_scale, id_a);
+            vs_a = load_scale(p.c.v_scale, id_a);
         }
         auto page_id = [&](int pg) {
             const int i = pg - page0;
-            const int a = __shfl_sync(0xffffffffu, id_a, i & 31), b = __shfl_sync(0xffffffffu, id_b, i & 31);
-            return i < 32 ? a : b;
+            return __shfl_sync(0xffffffffu, i < 32 ? id_a : id_b, i & 31);
         };
         auto issue = [&](int step) {   // whole warp; step of this run
             const int key = key0 + step * kStep;
@@ -278,19 +290,20 @@ __global__ void __launch_bounds__(Cfg<DIM>::kWarps * 32, 1)
         };
         for (int i = 0; i < C::kStages && i < n_steps; ++i) issue(i);
 
-        // queries: row r of the tile is new token r / group, head r % group
-        uint32_t qa[kTiles / 2][4];
-        float qscale[kHalves];
-        int row_lo[kHalves], row_hi[kHalves], lo_max = 0, hi_min = key_hi;
+        // queries: row r of the item is new token r / group, head r % group; this lane loads rows g and
+        // g + 8 (the product's columns), and keeps the scores of rows 2t, 2t + 1, + 8
+        uint32_t qb[kHalves][kSteps][2];
+        float qscale[kHalves][2];
+        int row_lo[kHalves][2], row_hi[kHalves][2];
+        const bool vec = ((reinterpret_cast<uintptr_t>(p.a.q) | (p.a.q_token_stride * 2) | (p.a.q_head_stride * 2)) & 15) == 0;
 #pragma unroll
         for (int hf = 0; hf < kHalves; ++hf) {
             const int row = g + 8 * hf;
             const bool live = row < n_rows;
-            const int i = live ? row / group : 0;
-            const T* q = static_cast<const T*>(p.a.q) + static_cast<int64_t>(sp.first + i) * p.a.q_token_stride +
+            const T* q = static_cast<const T*>(p.a.q) +
+                         static_cast<int64_t>(sp.first + (live ? row / group : 0)) * p.a.q_token_stride +
                          static_cast<int64_t>(it.head * group + (live ? row % group : 0)) * p.a.q_head_stride + 16 * t;
             T v[DIM / 4];
-            const bool vec = ((reinterpret_cast<uintptr_t>(p.a.q) | (p.a.q_token_stride * 2) | (p.a.q_head_stride * 2)) & 15) == 0;
 #pragma unroll
             for (int c = 0; c < DIM / 64; ++c) {
                 if (!live) {
@@ -305,7 +318,7 @@ __global__ void __launch_bounds__(Cfg<DIM>::kWarps * 32, 1)
                 }
             }
             int shift = 0;
-            if (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+            if (!std::is_same<T, __half>::value) {
                 float amax = 0.f;
 #pragma unroll
                 for (int k = 0; k < DIM / 4; ++k) amax = fmaxf(amax, fabsf(to_f32(v[k])));
@@ -314,9 +327,9 @@ __global__ void __launch_bounds__(Cfg<DIM>::kWarps * 32, 1)
                 shift = row_shift(amax);
             }
             const float mul = exp2_int(shift);
-            qscale[hf] = p.a.scale * kLog2e * exp2_int(-shift);
+            const float qs = p.a.scale * kLog2e * exp2_int(-shift);
 #pragma unroll
-            for (int k = 0; k < kTiles / 2; ++k) {
+            for (int k = 0; k < kSteps; ++k) {
                 // MMA step k = 4 c + i: channels 64 c + 16 t + 4 i + {0, 1 | 2, 3}
                 __half2 h0, h1;
                 if (std::is_same<T, __half>::value) {
@@ -326,35 +339,28 @@ __global__ void __launch_bounds__(Cfg<DIM>::kWarps * 32, 1)
                     h0 = __floats2half2_rn(to_f32(v[4 * k]) * mul, to_f32(v[4 * k + 1]) * mul);
                     h1 = __floats2half2_rn(to_f32(v[4 * k + 2]) * mul, to_f32(v[4 * k + 3]) * mul);
                 }
-                qa[k][hf] = *reinterpret_cast<uint32_t*>(&h0);
-                qa[k][2 + hf] = *reinterpret_cast<uint32_t*>(&h1);
-                if (kHalves == 1) qa[k][1] = qa[k][3] = 0;
+                qb[hf][k][0] = *reinterpret_cast<uint32_t*>(&h0);
+                qb[hf][k][1] = *reinterpret_cast<uint32_t*>(&h1);
             }
-            seen_keys(p, sp, i, row_lo[hf], row_hi[hf]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                qscale[hf][e] = __shfl_sync(0xffffffffu, qs, 4 * (2 * t + e));
+                const int mine = 2 * t + e + 8 * hf;
+                seen_keys(p, sp, mine < n_rows ? mine / group : 0, row_lo[hf][e], row_hi[hf][e]);
+            }
         }
-        {   // keys that every row sees: [lo_max, hi_min)
-            int lo, hi;
-            seen_keys(p, sp, 0, lo, hi);
-            hi_min = hi;
-            seen_keys(p, sp, sp.n - 1, lo, hi);
-            lo_max = lo;
-        }
-        int any_lo, any_hi;   // keys that some row sees
-        {
-            int x;
-            seen_keys(p, sp, 0, any_lo, x);
-            seen_keys(p, sp, sp.n - 1, x, any_hi);
-        }
+        // keys that every row sees: [lo_max, hi_min), that some row sees: [any_lo, any_hi)
+        int lo_max, hi_min, any_lo, any_hi;
+        seen_keys(p, sp, 0, any_lo, hi_min);
+        seen_keys(p, sp, sp.n - 1, lo_max, any_hi);
 
-        float o[kTiles][2 * kHalves], m[kHalves], l[kHalves];
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-            for (int e = 0; e < 2 * kHalves; ++e) o[j][e] = 0.f;
+        float o[kHalves][kSteps][4], m[kHalves][2], l[kHalves][2];
 #pragma unroll
         for (int hf = 0; hf < kHalves; ++hf) {
-            m[hf] = -INFINITY;
-            l[hf] = 0.f;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) o[hf][j][0] = o[hf][j][1] = o[hf][j][2] = o[hf][j][3] = 0.f;
+            m[hf][0] = m[hf][1] = -INFINITY;
+            l[hf][0] = l[hf][1] = 0.f;
         }
 
         bool ok = true;
@@ -362,18 +368,24 @@ __global__ void __launch_bounds__(Cfg<DIM>::kWarps * 32, 1)
             const int key = key0 + step * kStep;
             if ((key >> log_page) - page0 >= 32) {
                 page0 += 32;
-                id_a = id_b, ks_a = ks_b, vs_a = vs_b;
-                load_pages(page0 + 32, id_b, ks_b, vs_b);
+                id_a = id_b;
+                id_b = load_id(page0 + 32 + lane);
+                ks_a = load_scale(p.c.k_scale, id_a);
+                vs_a = load_scale(p.c.v_scale, id_a);
             }
-            // scales of the two 16-key halves
-            float ks[2], vs[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int i = ((key + 16 * u) >> log_page) - page0;
-                const float ka = __shfl_sync(0xffffffffu, ks_a, i & 31), kb = __shfl_sync(0xffffffffu, ks_b, i & 31);
-                const float va = __shfl_sync(0xffffffffu, vs_a, i & 31), vb = __shfl_sync(0xffffffffu, vs_b, i & 31);
-                ks[u] = i < 32 ? ka : kb;
-                vs[u] = i < 32 ? va : vb;
+            // scales of the step's page, or of its two pages of 16
+            float ks[kTilesM];
+            int ve[kTilesM];
+            {
+                const int i = (key >> log_page) - page0;
+                ks[0] = __shfl_sync(0xffffffffu, ks_a, i);
+                ve[0] = stored_exp(__shfl_sync(0xffffffffu, vs_a, i));
+                ks[1] = ks[0];
+                ve[1] = ve[0];
+                if (page < kStep) {
+                    ks[1] = __shfl_sync(0xffffffffu, ks_a, i + 1);
+                    ve[1] = stored_exp(__shfl_sync(0xffffffffu, vs_a, i + 1));
+                }
             }
             const uint32_t st = used % C::kStages;
             const uint32_t kbase = ring + st * C::kStage, vbase = kbase + C::kHalf;
@@ -385,89 +397,106 @@ __global__ void __launch_bounds__(Cfg<DIM>::kWarps * 32, 1)
             }
 
             // ── scores ──
-            float s[4][4];
+            float s[kHalves][kTilesM][4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-                const int kk = 8 * n + key_of_col<DIM>(g);
+            for (int mt = 0; mt < kTilesM; ++mt) {
+#pragma unroll
+                for (int hf = 0; hf < kHalves; ++hf) s[hf][mt][0] = s[hf][mt][1] = s[hf][mt][2] = s[hf][mt][3] = 0.f;
 #pragma unroll
                 for (int c = 0; c < DIM / 64; ++c) {
-                    const uint32_t line = DIM == 128 ? kk : kk >> 1;
-                    const uint32_t piece = DIM == 128 ? t + 4 * c : (kk & 1) * 4 + t;
-                    const uint4 w = lds128(kbase + line * 128 + ((piece ^ (line & 7)) << 4));
-                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+                    uint32_t w[2][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mma16816(s[n], qa[4 * c + i], codes2(ww[i]), codes2(ww[i] >> 16));
+                    for (int u = 0; u < 2; ++u) {
+                        const int kk = 16 * mt + 8 * u + key_of_row<DIM>(g);
+                        const uint32_t line = DIM == 128 ? kk : kk >> 1;
+                        const uint32_t piece = DIM == 128 ? t + 4 * c : (kk & 1) * 4 + t;
+                        const uint4 x = lds128(kbase + line * 128 + ((piece ^ (line & 7)) << 4));
+                        w[u][0] = x.x, w[u][1] = x.y, w[u][2] = x.z, w[u][3] = x.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t a0 = codes2(w[0][i]), a1 = codes2(w[1][i]);
+                        const uint32_t a2 = codes2(w[0][i] >> 16), a3 = codes2(w[1][i] >> 16);
+#pragma unroll
+                        for (int hf = 0; hf < kHalves; ++hf)
+                            mma16816(s[hf][mt], a0, a1, a2, a3, qb[hf][4 * c + i][0], qb[hf][4 * c + i][1]);
+                    }
                 }
             }
             const bool whole = key >= lo_max && key + kStep <= hi_min;   // no row masks any key here
-            float ve[2], rv[2];
+            float top[kHalves][2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int e = stored_exp(vs[u]);
-                ve[u] = static_cast<float>(e);
-                rv[u] = exp2_int(-e);
-            }
-            float top[kHalves];
+            for (int hf = 0; hf < kHalves; ++hf)
 #pragma unroll
-            for (int hf = 0; hf < kHalves; ++hf) {
-                top[hf] = m[hf];
+                for (int e = 0; e < 2; ++e) {
+                    top[hf][e] = m[hf][e];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const float f = fminf(qscale[hf] * ks[n >> 1], 3.4e38f);
+                    for (int mt = 0; mt < kTilesM; ++mt) {
+                        const float f = fminf(qscale[hf][e] * ks[mt], 3.4e38f);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float x = fmaf(s[n][2 * hf + e], f, ve[n >> 1]);
-                        if (!whole) {
-                            const int j = key + 8 * n + key_of_col<DIM>(2 * t + e);
-                            if (j < row_lo[hf] || j >= row_hi[hf]) x = -INFINITY;
+                        for (int u = 0; u < 2; ++u) {
+                            float x = fmaf(s[hf][mt][2 * u + e], f, static_cast<float>(ve[mt]));
+                            if (!whole) {
+                                const int j = key + 16 * mt + 8 * u + key_of_row<DIM>(g);
+                                if (j < row_lo[hf][e] || j >= row_hi[hf][e]) x = -INFINITY;
+                            }
+                            s[hf][mt][2 * u + e] = x;
+                            top[hf][e] = fmaxf(top[hf][e], x);
                         }
-                        s[n][2 * hf + e] = x;
-                        top[hf] = fmaxf(top[hf], x);
                     }
                 }
-                top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 1));
-                top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 2));
-            }
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+                for (int hf = 0; hf < kHalves; ++hf)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) top[hf][e] = fmaxf(top[hf][e], __shfl_xor_sync(0xffffffffu, top[hf][e], d));
             bool moved = false;
 #pragma unroll
-            for (int hf = 0; hf < kHalves; ++hf) moved = moved || top[hf] > m[hf];
+            for (int hf = 0; hf < kHalves; ++hf) moved = moved || top[hf][0] > m[hf][0] || top[hf][1] > m[hf][1];
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                for (int hf = 0; hf < kHalves; ++hf) {
-                    const float corr = m[hf] == top[hf] ? 1.f : ex2_approx(m[hf] - top[hf]);
-                    m[hf] = top[hf];
-                    l[hf] *= corr;
+                for (int hf = 0; hf < kHalves; ++hf)
 #pragma unroll
-                    for (int j = 0; j < kTiles; ++j) {
-                        o[j][2 * hf] *= corr;
-                        o[j][2 * hf + 1] *= corr;
+                    for (int e = 0; e < 2; ++e) {
+                        const float corr = m[hf][e] == top[hf][e] ? 1.f : ex2_approx(m[hf][e] - top[hf][e]);
+                        m[hf][e] = top[hf][e];
+                        l[hf][e] *= corr;
+#pragma unroll
+                        for (int j = 0; j < kSteps; ++j) {
+                            o[hf][j][e] *= corr;
+                            o[hf][j][2 + e] *= corr;
+                        }
                     }
-                }
             }
-            uint32_t pa[2][4];
+            uint32_t pb[kHalves][kTilesM][2];
 #pragma unroll
             for (int hf = 0; hf < kHalves; ++hf) {
-                const float ref = m[hf] == -INFINITY ? 0.f : m[hf];   // nothing seen yet: every x is -inf
+                // nothing seen yet: every x is -inf
+                const float ref0 = m[hf][0] == -INFINITY ? 0.f : m[hf][0], ref1 = m[hf][1] == -INFINITY ? 0.f : m[hf][1];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const float p0 = ex2_approx(s[n][2 * hf] - ref), p1 = ex2_approx(s[n][2 * hf + 1] - ref);
-                    l[hf] = fmaf(p0 + p1, rv[n >> 1], l[hf]);
-                    const __half2 h = __floats2half2_rn(p0, p1);
-                    pa[n >> 1][2 * (n & 1) + hf] = *reinterpret_cast<const uint32_t*>(&h);
+                for (int mt = 0; mt < kTilesM; ++mt) {
+                    float p4[4];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        p4[2 * u] = ex2_approx(s[hf][mt][2 * u] - ref0);
+                        p4[2 * u + 1] = ex2_approx(s[hf][mt][2 * u + 1] - ref1);
+                        const __half2 h = __floats2half2_rn(p4[2 * u], p4[2 * u + 1]);
+                        pb[hf][mt][u] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
+                    }
+                    const float rv = exp2_int(-ve[mt]);
+                    l[hf][0] = fmaf(p4[0] + p4[2], rv, l[hf][0]);
+                    l[hf][1] = fmaf(p4[1] + p4[3], rv, l[hf][1]);
                 }
             }
-            if (kHalves == 1)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) pa[u][1] = pa[u][3] = 0;
 
             // ── output ──
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int mt = 0; mt < kTilesM; ++mt) {
                 uint32_t w[4][DIM / 32];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int kk = 16 * u + 8 * (i >> 1) + key_of_col<DIM>(2 * t + (i & 1));
+                    const int kk = 16 * mt + 8 * (i >> 1) + key_of_row<DIM>(2 * t + (i & 1));
                     const uint32_t line = DIM == 128 ? kk : kk >> 1;
                     if (DIM == 128) {
                         const uint4 q4 = lds128(vbase + line * 128 + ((g ^ (line & 7)) << 4));
@@ -483,18 +512,15 @@ __global__ void __launch_bounds__(Cfg<DIM>::kWarps * 32, 1)
                         for (int j = 0; j < DIM / 32; ++j) w[i][j] = 0;
                 }
 #pragma unroll
-                for (int j = 0; j < DIM / 32; ++j) {
-                    const uint32_t x01 = prmt(w[0][j], w[1][j], 0x5140), y01 = prmt(w[0][j], w[1][j], 0x7362);
-                    const uint32_t x23 = prmt(w[2][j], w[3][j], 0x5140), y23 = prmt(w[2][j], w[3][j], 0x7362);
-                    const uint32_t b01[4] = {codes2(x01), codes2(x01 >> 16), codes2(y01), codes2(y01 >> 16)};
-                    const uint32_t b23[4] = {codes2(x23), codes2(x23 >> 16), codes2(y23), codes2(y23 >> 16)};
+                for (int j = 0; j < DIM / 32; ++j) {   // channels (DIM / 8) g + 4 j + {0, 1 | 2, 3}
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        float d[4] = {o[4 * j + b][0], o[4 * j + b][1], 0.f, 0.f};
-                        if (kHalves == 2) d[2] = o[4 * j + b][2 * kHalves - 2], d[3] = o[4 * j + b][2 * kHalves - 1];
-                        mma16816(d, pa[u], b01[b], b23[b]);
-                        o[4 * j + b][0] = d[0], o[4 * j + b][1] = d[1];
-                        if (kHalves == 2) o[4 * j + b][2 * kHalves - 2] = d[2], o[4 * j + b][2 * kHalves - 1] = d[3];
+                    for (int b = 0; b < 2; ++b) {
+                        const uint32_t lo = prmt(w[0][j], w[1][j], b ? 0x7362 : 0x5140);
+                        const uint32_t hi = prmt(w[2][j], w[3][j], b ? 0x7362 : 0x5140);
+                        const uint32_t a0 = codes2(lo), a1 = codes2(lo >> 16), a2 = codes2(hi), a3 = codes2(hi >> 16);
+#pragma unroll
+                        for (int hf = 0; hf < kHalves; ++hf)
+                            mma16816(o[hf][2 * j + b], a0, a1, a2, a3, pb[hf][mt][0], pb[hf][mt][1]);
                     }
                 }
             }
@@ -502,125 +528,131 @@ __global__ void __launch_bounds__(Cfg<DIM>::kWarps * 32, 1)
             if (step + C::kStages < n_steps) issue(step + C::kStages);
         }
 
-        // ── the run's end: rows' sums over the four lanes that share them ──
+        // ── the run's end: rows' sums over the eight lanes that share them ──
         const bool all = s0 == 0 && s1 == it.steps;
         const int64_t slot = 2ll * worker + (at > worker * run ? 1 : 0);
 #pragma unroll
-        for (int hf = 0; hf < kHalves; ++hf) {
-            l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
-            l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
-            const int row = g + 8 * hf;
-            if (row >= n_rows) continue;
-            // columns 2t and 2t + 1 of tile j: channels kTiles (2t) + j and kTiles (2t + 1) + j
-            float x[2][kTiles];
+        for (int hf = 0; hf < kHalves; ++hf)
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) x[0][j] = o[j][2 * hf], x[1][j] = o[j][2 * hf + 1];
-            if (all) {
-                const int token = sp.first + row / group, head = it.head * group + row % group;
-                const float inv = l[hf] == 0.f ? 0.f : 1.f / l[hf];
-                store_row<T>(p, token, head, kTiles * 2 * t, x[0], kTiles, inv);
-                store_row<T>(p, token, head, kTiles * (2 * t + 1), x[1], kTiles, inv);
-                if (p.a.lse && t == 0)
-                    p.a.lse[static_cast<int64_t>(token) * p.a.q_heads + head] =
-                        l[hf] == 0.f ? -INFINITY : (m[hf] + log2f(l[hf])) * kLn2;
-            } else {
-                float* po = r.part + (slot * ROWS + row) * DIM + kTiles * 2 * t;
+            for (int e = 0; e < 2; ++e) {
+                float sum = l[hf][e];
 #pragma unroll
-                for (int j = 0; j < 2 * kTiles; j += 4)
-                    *reinterpret_cast<float4*>(po + j) =
-                        make_float4(x[j / kTiles][j % kTiles], x[j / kTiles][j % kTiles + 1], x[j / kTiles][j % kTiles + 2],
-                                    x[j / kTiles][j % kTiles + 3]);
-                if (t == 0)
-                    *reinterpret_cast<float2*>(r.part + 2ll * r.workers * ROWS * DIM + (slot * ROWS + row) * 2) =
-                        make_float2(m[hf], l[hf]);
+                for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const int row = 2 * t + e + 8 * hf;
+                if (row >= n_rows) continue;
+                float x[2 * kSteps];   // channels [2 kSteps g, + 2 kSteps)
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j) x[2 * j] = o[hf][j][e], x[2 * j + 1] = o[hf][j][2 + e];
+                if (all) {
+                    const int token = sp.first + row / group, head = it.head * group + row % group;
+                    store_row<T>(p, token, head, 2 * kSteps * g, x, sum == 0.f ? 0.f : 1.f / sum);
+                    if (p.a.lse && g == 0)
+                        p.a.lse[static_cast<int64_t>(token) * p.a.q_heads + head] =
+                            sum == 0.f ? -INFINITY : (m[hf][e] + log2f(sum)) * kLn2;
+                } else {
+                    float* po = r.part + (slot * ROWS + row) * DIM + 2 * kSteps * g;
+#pragma unroll
+                    for (int j = 0; j < 2 * kSteps; j += 4)
+                        *reinterpret_cast<float4*>(po + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                    if (g == 0)
+                        *reinterpret_cast<float2*>(r.part + 2ll * r.workers * ROWS * DIM + (slot * ROWS + row) * 2) =
+                            make_float2(m[hf][e], sum);
+                }
             }
-        }
         if (!ok) break;
         at = it.begin + s1;
     }
 }
 
-// Adds up the partial results of the items that more than one run worked on:
-// block w takes the item that starts in run w and goes on past it.  Eight
-// warps share the runs; each lane keeps DIM / 32 channels.
+// Adds up the partial results of the items that more than one run worked on,
+// a block an item, its warps shared out among the item's rows and of each row
+// among its runs.  Each lane keeps DIM / 32 channels.
+constexpr int kJoinMax = 32;   // warps
+
 template <typename T, int DIM, int ROWS>
-__global__ void __launch_bounds__(256) k_attend_join(const __grid_constant__ RowsParams r) {
+__global__ void __launch_bounds__(kJoinMax * 32) k_attend_join(const __grid_constant__ RowsParams r) {
     constexpr int kPer = DIM / 32;
-    __shared__ int prefix[kMaxSeqs + 1 + 16];
-    __shared__ float so[8][DIM], sl[8];
+    __shared__ int prefix[kMaxSeqs + 1 + kJoinMax];
+    __shared__ float so[kJoinMax][DIM], sl[kJoinMax];
     make_prefix(r, prefix, prefix + kMaxSeqs + 1);
     const AttendParams& p = r.p;
     const int heads = p.c.kv_heads, group = p.a.q_heads / heads;
-    const int64_t total = static_cast<int64_t>(prefix[r.seqs]) * heads;
-    const int64_t run = run_length(total, r.workers);
-    const int w0 = blockIdx.x;
-    const int64_t edge = (w0 + 1) * run;          // first step of the next run
-    Place it = {};
-    if (edge < total) it = place_of(prefix, r.seqs, heads, edge - 1);
+    const int seq = blockIdx.x / heads, head = blockIdx.x % heads, steps = prefix[seq + 1] - prefix[seq];
+    const int64_t run = run_length(static_cast<int64_t>(prefix[r.seqs]) * heads, r.workers);
+    const int64_t begin = static_cast<int64_t>(prefix[seq]) * heads + static_cast<int64_t>(head) * steps;
+    const int w0 = static_cast<int>(begin / run), w1 = static_cast<int>((begin + steps - 1) / run);
+    const int slot0 = begin > w0 * run ? 1 : 0;
+    const SeqSpan sp = attend_span(p, r.seq0 + seq);
     pdl_wait();   // the partial results are complete (and this kernel ends after the one before it)
-    if (edge >= total || it.begin < w0 * run || it.begin + it.steps <= edge) return;
-    const int w1 = static_cast<int>((it.begin + it.steps - 1) / run);
-    const int slot0 = it.begin > w0 * run ? 1 : 0;
-    const SeqSpan sp = attend_span(p, r.seq0 + it.seq);
+    if (steps == 0 || w0 == w1) return;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int rows = sp.n * group;
+    const int share = max(1, warps / rows);        // warps a row
+    const int at_once = warps / share;             // rows at once
     const float* ml = r.part + 2ll * r.workers * ROWS * DIM;
-    for (int row = 0; row < sp.n * group; ++row) {
+    for (int row0 = 0; row0 < rows; row0 += at_once) {
+        const int row = row0 + warp / share, mine = warp % share;
         auto slot = [&](int w) { return (2ll * w + (w == w0 ? slot0 : 0)) * ROWS + row; };
-        float m = -INFINITY;
-        for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, ml[slot(w) * 2]);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        const float ref = m == -INFINITY ? 0.f : m;
-        float l = 0.f, o[kPer];
+        float m = -INFINITY, l = 0.f, o[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-#pragma unroll 4
-        for (int w = w0 + warp; w <= w1; w += 8) {
-            const float2 x = *reinterpret_cast<const float2*>(ml + slot(w) * 2);
-            const float f = ex2_approx(x.x - ref);
-            l = fmaf(x.y, f, l);
-            const float* po = r.part + slot(w) * DIM + lane * kPer;
-            float v[kPer];
-            if (kPer == 4) {
-                const float4 y = *reinterpret_cast<const float4*>(po);
-                v[0] = y.x, v[1] = y.y, v[kPer - 2] = y.z, v[kPer - 1] = y.w;
-            } else {
-                const float2 y = *reinterpret_cast<const float2*>(po);
-                v[0] = y.x, v[1] = y.y;
+        const bool live = row < rows && warp / share < at_once;
+        if (live) {
+            for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, ml[slot(w) * 2]);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 8
+            for (int w = w0 + mine; w <= w1; w += share) {
+                const float2 x = *reinterpret_cast<const float2*>(ml + slot(w) * 2);
+                const float f = ex2_approx(x.x - ref);
+                l = fmaf(x.y, f, l);
+                const float* po = r.part + slot(w) * DIM + lane * kPer;
+                float v[kPer];
+                if (kPer == 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(po);
+                    v[0] = y.x, v[1] = y.y, v[kPer - 2] = y.z, v[kPer - 1] = y.w;
+                } else {
+                    const float2 y = *reinterpret_cast<const float2*>(po);
+                    v[0] = y.x, v[1] = y.y;
+                }
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) o[i] = fmaf(v[i], f, o[i]);
             }
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) o[i] = fmaf(v[i], f, o[i]);
         }
+        if (share > 1) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) so[warp][lane * kPer + i] = o[i];
-        if (lane == 0) sl[warp] = l;
-        __syncthreads();
-        if (static_cast<int>(threadIdx.x) < DIM) {
-            float a = 0.f;
-            l = 0.f;
+            for (int i = 0; i < kPer; ++i) so[warp][lane * kPer + i] = o[i];
+            if (lane == 0) sl[warp] = l;
+            __syncthreads();
+            if (live && mine == 0)
+                for (int w = 1; w < share; ++w) {
 #pragma unroll
-            for (int w = 0; w < 8; ++w) {
-                a += so[w][threadIdx.x];
-                l += sl[w];
-            }
-            const int token = sp.first + row / group, head = it.head * group + row % group;
-            const int64_t at = static_cast<int64_t>(token) * p.a.q_heads + head;
-            from_f32(l == 0.f ? 0.f : a / l, static_cast<T*>(p.a.out)[at * DIM + threadIdx.x]);
-            if (p.a.lse && threadIdx.x == 0) p.a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+                    for (int i = 0; i < kPer; ++i) o[i] += so[warp + w][lane * kPer + i];
+                    l += sl[warp + w];
+                }
+            __syncthreads();
         }
-        __syncthreads();
+        if (live && mine == 0) {
+            const int token = sp.first + row / group, q_head = head * group + row % group;
+            const int64_t at = static_cast<int64_t>(token) * p.a.q_heads + q_head;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) from_f32(o[i] * inv, static_cast<T*>(p.a.out)[at * DIM + lane * kPer + i]);
+            if (p.a.lse && lane == 0) p.a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        }
     }
 }
 
 template <int DIM>
-int workers_of() { return device_sms() * Cfg<DIM>::kWarps; }
+int workers_of(int rows) { return device_sms() * (rows == 8 ? Cfg<DIM, 8>::kWarps : Cfg<DIM, 16>::kWarps); }
 
 int row_capacity(const AttendParams& p) { return p.a.max_q * (p.a.q_heads / p.c.kv_heads) <= 8 ? 8 : 16; }
 
 template <typename T, int DIM, int ROWS>
 int launch(const AttendParams& p, void* workspace, cudaStream_t st) {
-    using C = Cfg<DIM>;
+    using C = Cfg<DIM, ROWS>;
     static PerDeviceOnce smem_once;
     int rc = set_smem_limit_once(smem_once, k_attend_rows<T, DIM, ROWS>, C::kSmem, "cudaFuncSetAttribute(k_attend_rows)");
     if (rc) return rc;
@@ -630,7 +662,7 @@ int launch(const AttendParams& p, void* workspace, cudaStream_t st) {
     rc = make_map_2d(&mk, p.c.k, kMapU8, 128, lines, 128, 128, box, true);
     if (!rc) rc = make_map_2d(&mv, p.c.v, kMapU8, 128, lines, 128, 128, box, true);
     if (rc) return rc;
-    RowsParams r{p, 0, 0, workers_of<DIM>(), ROWS, static_cast<float*>(workspace)};
+    RowsParams r{p, 0, 0, workers_of<DIM>(ROWS), ROWS, static_cast<float*>(workspace)};
     // sequences a launch: the prefix array's room, and all their steps in 31 bits
     const int64_t most = static_cast<int64_t>(p.b.table_width) * p.c.page_tokens / kStep + 1;
     const int at_once = static_cast<int>(std::min<int64_t>(kMaxSeqs, 0x7fffffffll / most));
@@ -640,8 +672,10 @@ int launch(const AttendParams& p, void* workspace, cudaStream_t st) {
         cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return set_cuda_error("k_attend_rows", e);
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(r.workers);
-        cfg.blockDim = dim3(256);
+        const int items = r.seqs * p.c.kv_heads;
+        cfg.gridDim = dim3(items);
+        // few items are cut into many runs each: more warps to read them
+        cfg.blockDim = dim3(32 * (items > 4 * device_sms() ? 4 : items > device_sms() ? 8 : kJoinMax));
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -664,8 +698,9 @@ int launch_type(const AttendParams& p, void* workspace, cudaStream_t st) {
 }  // namespace
 
 int64_t attend_rows_workspace(const AttendParams& p) {
-    const int64_t workers = p.c.head_dim == 128 ? workers_of<128>() : workers_of<64>();
-    return workers * 2 * row_capacity(p) * (p.c.head_dim + 2) * 4;
+    const int rows = row_capacity(p);
+    const int64_t workers = p.c.head_dim == 128 ? workers_of<128>(rows) : workers_of<64>(rows);
+    return workers * 2 * rows * (p.c.head_dim + 2) * 4;
 }
 
 int launch_attend_rows(const AttendParams& p, void* workspace, cudaStream_t st) {
