@@ -73,8 +73,61 @@ __device__ __forceinline__ void seen_keys(const AttendParams& p, const SeqSpan& 
     }
 }
 
+// One query row by one warp in plain arithmetic, a key at a time: the keys of
+// [k0, k1) that the row sees, m in the units above, o and l against it, o in
+// DIM / 32 channels a lane.  A masked key does not touch the row, whatever it
+// holds; in the tensor cores' sums 0 * NaN of a value that other rows see is
+// NaN, so rows whose output came out NaN are taken again by this.
+template <typename T, int DIM>
+__device__ __noinline__ void attend_row_exact(const AttendParams& p, int seq, int token, int i, int q_head, int k0, int k1,
+                                              float (&o)[DIM / 32], float& m, float& l) {
+    constexpr int kPer = DIM / 32;
+    const int lane = threadIdx.x & 31, page = p.c.page_tokens, kv_head = q_head / (p.a.q_heads / p.c.kv_heads);
+    const SeqSpan sp = attend_span(p, seq);
+    int lo, hi;
+    seen_keys(p, sp, i, lo, hi);
+    const T* q = static_cast<const T*>(p.a.q) + token * p.a.q_token_stride + q_head * p.a.q_head_stride + lane * kPer;
+    float x[kPer];
+    for (int c = 0; c < kPer; ++c) {
+        x[c] = to_f32(q[c]) * (p.a.scale * kLog2e);
+        o[c] = 0.f;
+    }
+    m = -INFINITY;
+    l = 0.f;
+    for (int j = max(lo, k0); j < min(hi, k1); ++j) {
+        int id = __ldg(p.b.page_table + seq * p.b.table_stride + j / page);
+        if (id < 0 || id >= p.c.pages) id = 0;   // flagged where it was met first
+        const int64_t slab = static_cast<int64_t>(id) * p.c.kv_heads + kv_head;
+        const int64_t at = (slab * page + j % page) * DIM + lane * kPer;
+        float dot = 0.f;
+        for (int c = 0; c < kPer; c += 2) {
+            const float2 k = __half22float2(decode2(*reinterpret_cast<const uint16_t*>(p.c.k + at + c)));
+            dot = fmaf(x[c], k.x, fmaf(x[c + 1], k.y, dot));
+        }
+        for (int w = 16; w; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
+        const int ve = stored_exp(p.c.v_scale[slab]);
+        dot = fmaf(dot, p.c.k_scale[slab], static_cast<float>(ve));
+        const float top = fmaxf(m, dot), ref = top == -INFINITY ? 0.f : top;
+        const float old = m == top ? 1.f : ex2_approx(m - top), e = ex2_approx(dot - ref);
+        l = fmaf(e, exp2_int(-ve), l * old);
+        for (int c = 0; c < kPer; c += 2) {
+            const float2 v = __half22float2(decode2(*reinterpret_cast<const uint16_t*>(p.c.v + at + c)));
+            o[c] = fmaf(e, v.x, o[c] * old);
+            o[c + 1] = fmaf(e, v.y, o[c + 1] * old);
+        }
+        m = top;
+    }
+}
+
+// The float of a finished row: o / l, zeros where nothing was seen.
+__device__ __forceinline__ float row_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
+
 // kv_attend_rows.cu: at most 16 query rows (new tokens x heads of a group) a key head.
 int64_t attend_rows_workspace(const AttendParams& p);
 int launch_attend_rows(const AttendParams& p, void* workspace, cudaStream_t st);
+// kv_attend_tiles.cu: any number of query rows, in tiles of 256.
+int64_t attend_tiles_workspace(const AttendParams& p);
+int launch_attend_tiles(const AttendParams& p, void* workspace, cudaStream_t st);
 
 }  // namespace b3

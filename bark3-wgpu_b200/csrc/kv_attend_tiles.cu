@@ -1,0 +1,750 @@
+// kv_attend_tiles.cu — attention over the paged 8-bit cache for many query
+// rows: prompts, chunks of prompts, decode steps with more than 16 rows a key
+// head.  The mathematics is in kv_attend.cuh.
+//
+// Bound by arithmetic: 4 head_dim operations a (row, key) pair on tcgen05 and
+// one exponential, of which an SM makes 16 a clock, as long as 512 (head_dim
+// 128) of its tensor operations.
+//
+// An item is 256 query rows (new token x head of the group, so K and V are
+// read, expanded and staged once for all heads that share them) of one key
+// head; it walks its keys in blocks of 128.  Its two halves of 128 rows take
+// turns: while the softmax warps of one work on a block's scores, the tensor
+// cores multiply for the other.
+//   warps 0..3, 4..7   softmax of half 0 and 1: a thread owns a row, so the
+//                      running maximum and sum need no exchange.  They stage
+//                      the half's queries (f16, 128-byte swizzle), read the
+//                      scores from TMEM twice (maximum, then exponentials),
+//                      write P (f16) over them, move the reference maximum only
+//                      when a row's grows by more than 2^8 (and then rescale O
+//                      in TMEM), and store the output.
+//   warps 8..14        expand codes to f16 operands: 16-byte loads of a page's
+//                      rows, one block ahead in registers, K and V both as
+//                      128-byte swizzled rows of 64 channels (K-major for S,
+//                      MN-major for PV).
+//   warp 15            one thread issues S = Q K^T (M128 N128 K128) and
+//                      O += P V (M128 N128 K128, P from TMEM).
+// TMEM: S/P of both halves 2 x 128 columns, O 2 x 128.
+//
+// Work.  k_attend_plan lists the items with their blocks; all blocks of all
+// (item, key head) pairs, laid end to end, are cut into equal runs, one a CTA,
+// so causal triangles, ragged prompts and few rows over many keys end
+// together.  A run that covers an item from end to end stores it, other runs
+// leave partial results that k_attend_tiles_join adds up in run order.
+#include <type_traits>
+
+#include "b3_ptx.cuh"
+#include "kv_attend.cuh"
+
+namespace b3 {
+namespace {
+
+constexpr int kRows = 256;          // query rows of an item
+constexpr int kKeys = 128;          // keys of a block
+// 16 warps, four on each scheduler: a 17th would cut every thread's registers from 128 to 96
+constexpr int kThreads = 512;
+constexpr int kExpWarp0 = 8, kExpWarps = 7, kMmaWarp = 15;
+constexpr int kMinRun = 2;          // blocks of a run at least
+constexpr float kMove = 8.f;        // log2: how far a maximum may pass the reference
+
+struct Tile {
+    int seq, first, n, len;         // sequence, its first query row, new tokens, cached tokens
+    int row0, steps, key_lo, pad;   // first query row of the item in the sequence, blocks, first key
+    int64_t begin, pad2;            // blocks (of one key head) of the items before
+};
+
+struct TilesParams {
+    AttendParams p;
+    int tiles;              // entries of `tile`; tile[tiles].begin is the total
+    int runs;
+    Tile* tile;
+    float* part;            // [runs][2][kRows][DIM], then [runs][2][kRows][2] (m, l)
+};
+
+template <int DIM>
+struct Cfg {
+    static constexpr uint32_t kHalf = kKeys * 128;               // 64 channels of 128 rows (keys or queries)
+    static constexpr uint32_t kOperand = kHalf * (DIM / 64);
+    static constexpr uint32_t kQ = 0;                            // 2 halves of rows
+    static constexpr uint32_t kK = 2 * kOperand;                 // 2 stages
+    static constexpr uint32_t kV = 4 * kOperand;                 // 2 stages
+    static constexpr uint32_t kBar = 6 * kOperand;
+    static constexpr uint32_t kSmem = kBar + 256 + 1024;
+    static constexpr uint32_t kTmemS = 0, kTmemO = 256;
+    static constexpr uint32_t kIdescS = idesc_f16_f32_b<128, 128, 0>();
+    static constexpr uint32_t kIdescPV = idesc_f16_f32_b<128, DIM, 1>();
+};
+
+// ───────────────────────────── the plan ─────────────────────────────
+
+__global__ void __launch_bounds__(1024) k_attend_plan(const __grid_constant__ TilesParams r) {
+    __shared__ int64_t sums[32];
+    const AttendParams& p = r.p;
+    const int group = p.a.q_heads / p.c.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();
+    int64_t carry = 0;
+    // items before sequence i's: cu_q[i] * group / kRows + i, room for every sequence's last, part-filled one
+    auto key = [&](int i) { return static_cast<int64_t>(__ldg(p.b.cu_q + i)) * group / kRows + i; };
+    for (int base = 0; base < r.tiles; base += 1024) {
+        const int u = base + tid;
+        Tile t = {};
+        if (u < r.tiles) {
+            int lo = 0, hi = p.b.n_seq;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (key(mid) <= u) lo = mid; else hi = mid;
+            }
+            const SeqSpan sp = attend_span(p, lo);
+            const int64_t row0 = (u - key(lo)) * kRows;
+            if (row0 >= 0 && row0 < static_cast<int64_t>(sp.n) * group) {
+                t.seq = lo, t.first = sp.first, t.n = sp.n, t.len = sp.len;
+                t.row0 = static_cast<int>(row0);
+                const int last = static_cast<int>(min(row0 + kRows, static_cast<int64_t>(sp.n) * group)) - 1;
+                int a, hi_key, lo_key;
+                seen_keys(p, sp, t.row0 / group, lo_key, a);
+                seen_keys(p, sp, last / group, a, hi_key);
+                t.key_lo = min(lo_key, hi_key) / kKeys * kKeys;
+                t.steps = max(1, (hi_key - t.key_lo + kKeys - 1) / kKeys);   // rows that see nothing are written too
+            }
+        }
+        int64_t v = t.steps;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, v, d);
+            if (lane >= d) v += x;
+        }
+        if (lane == 31) sums[warp] = v;
+        __syncthreads();
+        int64_t before = carry, all = carry;
+        for (int w = 0; w < 32; ++w) {
+            before += w < warp ? sums[w] : 0;
+            all += sums[w];
+        }
+        t.begin = before + v - t.steps;
+        if (u < r.tiles) r.tile[u] = t;
+        carry = all;
+        __syncthreads();
+    }
+    if (tid == 0) r.tile[r.tiles].begin = carry;
+}
+
+__device__ __forceinline__ int64_t run_length(int64_t total, int runs) {
+    return max(static_cast<int64_t>(kMinRun), (total + runs - 1) / runs);
+}
+
+// Walks the items of a run: [s0, s1) are the blocks of the item in it.
+struct Walk {
+    const Tile* tile;
+    int tiles, heads;
+    int64_t at, end, start;
+    int u, head, s0, s1;
+    Tile t;
+
+    // the whole warp; false where the run is empty
+    __device__ __forceinline__ bool init(const TilesParams& r, int run_id) {
+        tile = r.tile;
+        tiles = r.tiles;
+        heads = r.p.c.kv_heads;
+        const int64_t total = __ldg(&tile[tiles].begin) * heads, run = run_length(total, r.runs);
+        at = start = run_id * run;
+        end = min(at + run, total);
+        if (at >= end) return false;
+        // the last item that begins at or before `at` (items without blocks begin where the next one does)
+        const int lane = threadIdx.x & 31;
+        int lo = 0, len = tiles;
+        while (len > 1) {
+            const int step = (len + 31) >> 5, i = lane * step;
+            const unsigned m = __ballot_sync(0xffffffffu, i < len && __ldg(&tile[lo + i].begin) * heads <= at);
+            const int k = m ? (31 - __clz(m)) * step : 0;
+            lo += k;
+            len = min(step, len - k);
+        }
+        u = lo;
+        load();
+        const int64_t in = at - t.begin * heads;
+        head = static_cast<int>(in / t.steps);
+        set(static_cast<int>(in % t.steps));
+        return true;
+    }
+    __device__ __forceinline__ void load() {
+        const int4* q = reinterpret_cast<const int4*>(tile + u);
+        const int4 a = __ldg(q), b = __ldg(q + 1);
+        t.seq = a.x, t.first = a.y, t.n = a.z, t.len = a.w, t.row0 = b.x, t.steps = b.y, t.key_lo = b.z;
+        t.begin = __ldg(&tile[u].begin);
+    }
+    __device__ __forceinline__ void set(int from) {
+        s0 = from;
+        s1 = static_cast<int>(min(static_cast<int64_t>(t.steps), from + (end - at)));
+    }
+    __device__ __forceinline__ bool next() {
+        at += s1 - s0;
+        if (at >= end) return false;
+        if (++head == heads) {
+            head = 0;
+            do ++u; while (__ldg(&tile[u].steps) == 0);   // at < end: an item with blocks follows
+            load();
+        }
+        set(0);
+        return true;
+    }
+};
+
+// ───────────────────────────── the kernel ─────────────────────────────
+
+__device__ __forceinline__ uint32_t h2u(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_constant__ TilesParams r) {
+    using C = Cfg<DIM>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const AttendParams& p = r.p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // Barriers.  k, v: two stages each, phases over the CTA's blocks; q: a half's
+    // queries are staged (an item); s: a half's scores are in TMEM, p: its
+    // probabilities are (a block); o: its last product is done (an item).
+    const uint32_t bars = smem_u32(smem + C::kBar);
+    auto k_full = [&](int s) { return bars + 8 * s; };
+    auto k_empty = [&](int s) { return bars + 16 + 8 * s; };
+    auto v_full = [&](int s) { return bars + 32 + 8 * s; };
+    auto v_empty = [&](int s) { return bars + 48 + 8 * s; };
+    auto q_full = [&](int h) { return bars + 64 + 8 * h; };
+    auto s_full = [&](int h) { return bars + 80 + 8 * h; };
+    auto p_full = [&](int h) { return bars + 96 + 8 * h; };
+    auto o_full = [&](int h) { return bars + 112 + 8 * h; };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBar + 128);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(k_full(i), kExpWarps);
+            mbar_init(v_full(i), kExpWarps);
+            mbar_init(k_empty(i), 1);
+            mbar_init(v_empty(i), 1);
+            mbar_init(q_full(i), 4);
+            mbar_init(s_full(i), 1);
+            mbar_init(p_full(i), 4);
+            mbar_init(o_full(i), 1);
+        }
+        fence_mbar_init();
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc<512>(smem_u32(tmem_slot));
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
+    pdl_wait();   // the plan is complete
+
+    const int group = p.a.q_heads / p.c.kv_heads, heads = p.c.kv_heads, page = p.c.page_tokens;
+    const int log_page = 31 - __clz(page);
+    Walk w;
+    const bool any = w.init(r, blockIdx.x);
+    auto halves = [&]() { return w.t.n * group - w.t.row0 > 128 ? 2 : 1; };
+    bool ok = any;
+
+    if (!any) {
+        // no run for this CTA
+    } else if (warp == kMmaWarp) {
+        // ── MMA issuer ──
+        if (lane == 0) {
+            const uint32_t sq = smem_u32(smem + C::kQ), sk = smem_u32(smem + C::kK), sv = smem_u32(smem + C::kV);
+            uint32_t g = 0, items[2] = {0, 0}, blocks[2] = {0, 0};   // blocks of the CTA; items and blocks of each half
+            auto scores = [&](int h, uint32_t gb) {   // S of half h for the CTA's block gb
+                const uint64_t a0 = smem_desc_sw128(sq + h * C::kOperand), b0 = smem_desc_sw128(sk + (gb & 1) * C::kOperand);
+#pragma unroll
+                for (int k = 0; k < DIM / 16; ++k) {
+                    const uint32_t off = (k >> 2) * C::kHalf + (k & 3) * 32;
+                    mma_f16_ss(tmem + C::kTmemS + 128 * h, desc_advance(a0, off), desc_advance(b0, off), C::kIdescS, k > 0);
+                }
+                mma_commit(s_full(h));
+            };
+            do {
+                const int nh = halves(), n = w.s1 - w.s0;
+                for (int h = 0; h < nh && ok; ++h) {
+                    ok = mbar_wait(q_full(h), items[h] & 1, 0x70);
+                    ++items[h];
+                    if (ok && h == 0) ok = mbar_wait(k_full(g & 1), (g >> 1) & 1, 0x71);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(h, g);
+                }
+                if (ok) mma_commit(k_empty(g & 1));
+                for (int j = 0; j < n && ok; ++j, ++g) {
+                    const uint32_t st = g & 1;
+                    for (int h = 0; h < nh && ok; ++h) {
+                        ok = mbar_wait(p_full(h), blocks[h] & 1, 0x72);
+                        ++blocks[h];
+                        if (ok && h == 0) ok = mbar_wait(v_full(st), (g >> 1) & 1, 0x73);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t bv = smem_desc_sw128_mn(sv + st * C::kOperand, C::kHalf, 1024);
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k)
+                            mma_f16_ts(tmem + C::kTmemO + 128 * h, tmem + C::kTmemS + 128 * h + 8 * k, desc_advance(bv, 2048 * k),
+                                       C::kIdescPV, j > 0 || k > 0);
+                        if (h == nh - 1) mma_commit(v_empty(st));
+                        if (j == n - 1) mma_commit(o_full(h));
+                        if (j + 1 < n) {
+                            if (h == 0) {
+                                ok = mbar_wait(k_full((g + 1) & 1), ((g + 1) >> 1) & 1, 0x74);
+                                if (!ok) break;
+                                tc_fence_after();
+                            }
+                            scores(h, g + 1);   // over P of this block: the products run in order
+                            if (h == nh - 1) mma_commit(k_empty((g + 1) & 1));
+                        }
+                    }
+                }
+            } while (ok && w.next());
+            if (!ok) kv_flag(p.c.status, B3_KV_TIMEOUT);
+        }
+    } else if (warp >= kExpWarp0) {
+        // ── codes to f16 operands ──
+        // a warp's loads cover four keys x 128 bytes (eight x 64): a lane takes 16 bytes, lanes of
+        // a quarter-warp four pieces of 64 channels of two keys, so that the swizzled 16-byte
+        // stores of each quarter touch every bank once
+        constexpr int kKeysWarp = 512 / DIM;               // keys of one load of a warp
+        constexpr int kPass = kExpWarps * kKeysWarp;       // keys of one load of all warps
+        constexpr int kLoads = (kKeys + kPass - 1) / kPass;   // loads a thread and operand (the last for some warps)
+        const int ew = warp - kExpWarp0;
+        const int piece = DIM == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;   // 16 channels
+        const int sub = DIM == 128 ? ((lane >> 2) & 1) + 2 * (lane >> 4) : lane >> 2;
+        const int row = ew * kKeysWarp + sub;              // + i * kPass
+        uint4 kc[kLoads], vc[kLoads];
+        int any_lo, any_hi;       // keys that some row of the item sees
+        const int32_t* pages;
+        auto item = [&]() {
+            const SeqSpan sp = {w.t.first, w.t.n, w.t.len};
+            const int last = min(w.t.row0 + kRows, w.t.n * group) - 1;
+            int x;
+            seen_keys(p, sp, w.t.row0 / group, any_lo, x);
+            seen_keys(p, sp, last / group, x, any_hi);
+            pages = p.b.page_table + w.t.seq * p.b.table_stride;
+        };
+        auto load = [&](const uint8_t* codes, uint4 (&c)[kLoads], int block) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int key = w.t.key_lo + block * kKeys + row + i * kPass;
+                c[i] = make_uint4(0, 0, 0, 0);   // a key that no row sees: 0, whatever its place holds
+                if (row + i * kPass < kKeys && key >= any_lo && key < any_hi) {
+                    int id = __ldg(pages + (key >> log_page));
+                    if (id < 0 || id >= p.c.pages) {
+                        kv_flag(p.c.status, B3_KV_BAD_PAGE);
+                        id = 0;
+                    }
+                    const int64_t line = (static_cast<int64_t>(id) * heads + w.head) * page + (key & (page - 1));
+                    c[i] = __ldg(reinterpret_cast<const uint4*>(codes + line * DIM + 16 * piece));
+                }
+            }
+        };
+        auto expand = [&](uint8_t* to, const uint4 (&c)[kLoads]) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int key = row + i * kPass;
+                if (key >= kKeys) break;
+                uint8_t* line = to + (piece >> 2) * C::kHalf + key * 128;
+                const uint32_t in[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+                uint32_t out[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const __half2 a = decode2(in[k] & 0xffffu), b = decode2(in[k] >> 16);
+                    out[2 * k] = *reinterpret_cast<const uint32_t*>(&a);
+                    out[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&b);
+                }
+                const int c0 = 2 * (piece & 3), sw = key & 7;
+                *reinterpret_cast<uint4*>(line + ((c0 ^ sw) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+                *reinterpret_cast<uint4*>(line + (((c0 + 1) ^ sw) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+            }
+            fence_async_shared();
+            __syncwarp();
+        };
+        uint32_t g = 0;
+        item();
+        load(p.c.k, kc, w.s0);
+        load(p.c.v, vc, w.s0);
+        bool more = true;
+        while (ok && more) {
+            // this block is in registers; the next one (of this item or the next) is loaded behind it
+            const uint32_t st = g & 1;
+            if (g >= 2) ok = __all_sync(0xffffffffu, mbar_wait(k_empty(st), ((g >> 1) - 1) & 1, 0x75));
+            if (!ok) break;
+            expand(smem + C::kK + st * C::kOperand, kc);
+            if (lane == 0) mbar_arrive(k_full(st));
+            const int j = w.s0;
+            if (j + 1 < w.s1) {
+                ++w.s0, ++w.at;   // Walk::next adds what is left
+            } else {
+                more = w.next();
+                if (more) item();
+            }
+            if (more) load(p.c.k, kc, w.s0);
+            if (g >= 2) ok = __all_sync(0xffffffffu, mbar_wait(v_empty(st), ((g >> 1) - 1) & 1, 0x76));
+            if (!ok) break;
+            expand(smem + C::kV + st * C::kOperand, vc);
+            if (lane == 0) mbar_arrive(v_full(st));
+            if (more) load(p.c.v, vc, w.s0);
+            ++g;
+        }
+        if (!ok && lane == 0) kv_flag(p.c.status, B3_KV_TIMEOUT);
+    } else {
+        // ── softmax: half h, a row a thread ──
+        const int h = warp >> 2, mine = (warp & 3) * 32 + lane;
+        const uint32_t lrow = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lrow + C::kTmemS + 128 * h, to = tmem + lrow + C::kTmemO + 128 * h;
+        uint8_t* sq = smem + C::kQ + h * C::kOperand + mine * 128;
+        const bool vec = ((reinterpret_cast<uintptr_t>(p.a.q) | (p.a.q_token_stride * 2) | (p.a.q_head_stride * 2)) & 15) == 0;
+        float qscale = 0.f;
+        // stages this thread's query row of the walk's item
+        auto stage = [&]() {
+            const int row = w.t.row0 + 128 * h + mine;
+            const bool live = row < w.t.n * group;
+            const T* q = static_cast<const T*>(p.a.q) + static_cast<int64_t>(w.t.first + (live ? row / group : 0)) * p.a.q_token_stride +
+                         static_cast<int64_t>(w.head * group + (live ? row % group : 0)) * p.a.q_head_stride;
+            auto piece = [&](int c, float (&x)[8]) {
+                if (vec)
+                    load8<true>(q + 8 * c, x);
+                else
+                    load8<false>(q + 8 * c, x);
+            };
+            const float sign = p.a.scale < 0.f ? -1.f : 1.f;   // scores are scaled by what is positive: order is kept
+            int shift = 0;
+            if (live && !std::is_same<T, __half>::value) {
+                float amax = 0.f;
+                for (int c = 0; c < DIM / 8; ++c) {
+                    float x[8];
+                    piece(c, x);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+                }
+                shift = row_shift(amax);
+            }
+            const float mul = sign * exp2_int(shift);
+            qscale = fabsf(p.a.scale) * kLog2e * exp2_int(-shift);
+#pragma unroll 4
+            for (int c = 0; c < DIM / 8; ++c) {
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (live) piece(c, x);
+                *reinterpret_cast<uint4*>(sq + (c >> 3) * C::kHalf + (((c & 7) ^ (mine & 7)) << 4)) =
+                    make_uint4(h2u(x[0] * mul, x[1] * mul), h2u(x[2] * mul, x[3] * mul), h2u(x[4] * mul, x[5] * mul),
+                               h2u(x[6] * mul, x[7] * mul));
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full(h));
+        };
+        uint32_t items = 0, blocks = 0;
+        bool more = true, mine_next = halves() > h;
+        if (mine_next) stage();
+        while (ok && more) {
+            if (!mine_next) {   // an item without a second half
+                more = w.next();
+                mine_next = more && halves() > h;
+                if (mine_next) stage();
+                continue;
+            }
+            const Tile t = w.t;
+            const int head = w.head, s0 = w.s0, s1 = w.s1;
+            const SeqSpan sp = {t.first, t.n, t.len};
+            const int rows = min(128, t.n * group - t.row0 - 128 * h);
+            const int row = t.row0 + 128 * h + min(mine, rows - 1);
+            int row_lo, row_hi, lo_max, hi_min, x;
+            seen_keys(p, sp, row / group, row_lo, row_hi);
+            seen_keys(p, sp, (t.row0 + 128 * h) / group, x, hi_min);
+            seen_keys(p, sp, (t.row0 + 128 * h + rows - 1) / group, lo_max, x);
+            int any_lo, any_hi;
+            seen_keys(p, sp, t.row0 / group, any_lo, x);
+            seen_keys(p, sp, (min(t.row0 + kRows, t.n * group) - 1) / group, x, any_hi);
+            const int32_t* pages = p.b.page_table + t.seq * p.b.table_stride;
+            // lane i (0..7) brings the scales of the block's keys [16 i, 16 i + 16)
+            auto scales = [&](int block, float& ks, int& ve) {
+                const int key = t.key_lo + block * kKeys + 16 * (lane & 7);
+                ks = 1.f;
+                ve = 0;
+                if (block < s1 && key + 16 > any_lo && key < any_hi) {
+                    int id = __ldg(pages + (key >> log_page));
+                    if (id < 0 || id >= p.c.pages) id = 0;   // flagged by the expanding warps
+                    ks = __ldg(p.c.k_scale + static_cast<int64_t>(id) * heads + head);
+                    ve = stored_exp(__ldg(p.c.v_scale + static_cast<int64_t>(id) * heads + head));
+                }
+            };
+            float ks, ks_next;
+            int ve, ve_next;
+            scales(s0, ks_next, ve_next);
+            float m = -INFINITY, l = 0.f;
+            const float qs = qscale;
+            for (int j = s0; j < s1; ++j) {
+                ks = ks_next, ve = ve_next;
+                scales(j + 1, ks_next, ve_next);
+                ok = __all_sync(0xffffffffu, mbar_wait(s_full(h), blocks & 1, 0x77));
+                ++blocks;
+                if (!ok) break;
+                tc_fence_after();
+                const int key = t.key_lo + j * kKeys;
+                const bool whole = key >= lo_max && key + kKeys <= hi_min;
+                // maximum: of the raw products in each 16 keys, then scaled (the factor is positive)
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t a[32];
+                    tmem_ld_32x32b_x32(ts + 32 * c, a);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int at = 2 * c + u;
+                        const float f = fminf(qs * __shfl_sync(0xffffffffu, ks, at), 3.4e38f);
+                        const float e = static_cast<float>(__shfl_sync(0xffffffffu, ve, at));
+                        float g0 = -INFINITY, g1 = -INFINITY;
+                        if (whole) {
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                g0 = fmaxf(g0, __uint_as_float(a[16 * u + i]));
+                                g1 = fmaxf(g1, __uint_as_float(a[16 * u + i + 1]));
+                            }
+                        } else {
+                            const int k0 = key + 16 * at;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if (k0 + i >= row_lo && k0 + i < row_hi) g0 = fmaxf(g0, __uint_as_float(a[16 * u + i]));
+                        }
+                        g0 = fmaxf(g0, g1);
+                        if (g0 > -INFINITY) top = fmaxf(top, fmaf(g0, f, e));
+                    }
+                }
+                const bool grow = top > m + kMove || (m == -INFINITY && top > -INFINITY);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float m_new = grow ? top : m;
+                    const float corr = m_new == m ? 1.f : ex2_approx(m - m_new);
+                    m = m_new;
+                    l *= corr;
+                    if (j > s0) {   // the products so far are done: S was issued after them
+#pragma unroll
+                        for (int c = 0; c < DIM / 32; ++c) {
+                            uint32_t a[32];
+                            tmem_ld_32x32b_x32(to + 32 * c, a);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * corr);
+                            tmem_st_32x32b_x32(to + 32 * c, a);
+                        }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t a[32], b[16];
+                    tmem_ld_32x32b_x32(ts + 32 * c, a);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int at = 2 * c + u;
+                        const float f = fminf(qs * __shfl_sync(0xffffffffu, ks, at), 3.4e38f);
+                        const int ei = __shfl_sync(0xffffffffu, ve, at);
+                        const float e = static_cast<float>(ei) - ref;
+                        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            float2 y = __ffma2_rn(make_float2(__uint_as_float(a[16 * u + i]), __uint_as_float(a[16 * u + i + 1])),
+                                                  make_float2(f, f), make_float2(e, e));
+                            if (!whole) {
+                                const int k0 = key + 16 * at + i;
+                                if (k0 < row_lo || k0 >= row_hi) y.x = -INFINITY;
+                                if (k0 + 1 < row_lo || k0 + 1 >= row_hi) y.y = -INFINITY;
+                            }
+                            y = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                            sum = __fadd2_rn(sum, y);
+                            b[8 * u + (i >> 1)] = h2u(y.x, y.y);
+                        }
+                        l = fmaf(sum.x + sum.y, exp2_int(-ei), l);
+                    }
+                    tmem_st_32x32b_x16(ts + 16 * c, b);   // over scores that were read
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(h));
+            }
+            if (!ok) break;
+            // the next item's queries, then this one's output
+            const int64_t slot = 2ll * blockIdx.x + (w.at > w.start ? 1 : 0);
+            more = w.next();
+            mine_next = more && halves() > h;
+            if (mine_next) stage();
+            ok = __all_sync(0xffffffffu, mbar_wait(o_full(h), items & 1, 0x78));
+            ++items;
+            if (!ok) break;
+            tc_fence_after();
+            const bool all = s0 == 0 && s1 == t.steps, live = mine < rows;
+            const int token = t.first + row / group, q_head = head * group + row % group;
+            const float inv = row_inverse(l);
+            T* out = static_cast<T*>(p.a.out) + (static_cast<int64_t>(token) * p.a.q_heads + q_head) * DIM;
+            float* po = r.part + (slot * kRows + 128 * h + mine) * DIM;
+            float* ml = r.part + 2ll * r.runs * kRows * DIM + (slot * kRows + 128 * h + mine) * 2;
+            float nan = 0.f;
+#pragma unroll
+            for (int c = 0; c < DIM / 32; ++c) {
+                uint32_t a[32];
+                tmem_ld_32x32b_x32(to + 32 * c, a);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) nan = fmaf(__uint_as_float(a[i]), 0.f, nan);
+                if (live && all) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        float x8[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) x8[k] = __uint_as_float(a[i + k]) * inv;
+                        store8(out + 32 * c + i, x8);
+                    }
+                } else if (live) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<uint4*>(po + 32 * c + i) = make_uint4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+                }
+            }
+            tc_fence_before();
+            if (live && all) {
+                if (p.a.lse) p.a.lse[static_cast<int64_t>(token) * p.a.q_heads + q_head] = row_lse(m, l);
+            } else if (live) {
+                *reinterpret_cast<float2*>(ml) = make_float2(m, l);
+            }
+            // rows that came out NaN (or infinite): again, without the keys they do not see
+            unsigned bad = __ballot_sync(0xffffffffu, live && nan != nan);
+            while (bad) {
+                const int src = __ffs(bad) - 1;
+                bad &= bad - 1;
+                const int rr = t.row0 + 128 * h + (warp & 3) * 32 + src;
+                const int tok = t.first + rr / group, qh = head * group + rr % group;
+                float o[DIM / 32], mm, ll;
+                attend_row_exact<T, DIM>(p, t.seq, tok, rr / group, qh, t.key_lo + s0 * kKeys, t.key_lo + s1 * kKeys, o, mm, ll);
+                if (all) {
+                    const int64_t at = static_cast<int64_t>(tok) * p.a.q_heads + qh;
+                    for (int c = 0; c < DIM / 32; ++c)
+                        from_f32(o[c] * row_inverse(ll), static_cast<T*>(p.a.out)[at * DIM + lane * (DIM / 32) + c]);
+                    if (p.a.lse && lane == 0) p.a.lse[at] = row_lse(mm, ll);
+                } else {
+                    const int64_t at = slot * kRows + rr - t.row0;
+                    for (int c = 0; c < DIM / 32; ++c) r.part[at * DIM + lane * (DIM / 32) + c] = o[c];
+                    if (lane == 0)
+                        *reinterpret_cast<float2*>(r.part + 2ll * r.runs * kRows * DIM + at * 2) = make_float2(mm, ll);
+                }
+            }
+        }
+        if (!ok && lane == 0) kv_flag(p.c.status, B3_KV_TIMEOUT);
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc<512>(tmem);
+    }
+}
+
+// Adds up partial results: block (w, y) takes 32 rows of the item that starts
+// in run w and goes on past it.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(256) k_attend_tiles_join(const __grid_constant__ TilesParams r) {
+    constexpr int kPer = DIM / 32;
+    const AttendParams& p = r.p;
+    pdl_wait();
+    const int heads = p.c.kv_heads, group = p.a.q_heads / heads;
+    const int64_t total = __ldg(&r.tile[r.tiles].begin) * heads, run = run_length(total, r.runs);
+    const int w0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t edge = (w0 + 1) * run;
+    if (edge >= total) return;
+    const int64_t want = edge - 1;
+    int lo = 0, len = r.tiles;
+    while (len > 1) {
+        const int step = (len + 31) >> 5, i = lane * step;
+        const unsigned m = __ballot_sync(0xffffffffu, i < len && __ldg(&r.tile[lo + i].begin) * heads <= want);
+        const int k = m ? (31 - __clz(m)) * step : 0;
+        lo += k;
+        len = min(step, len - k);
+    }
+    const Tile t = r.tile[lo];
+    const int head = static_cast<int>((want - t.begin * heads) / t.steps);
+    const int64_t begin = t.begin * heads + static_cast<int64_t>(head) * t.steps;
+    if (begin < w0 * run || begin + t.steps <= edge) return;
+    const int w1 = static_cast<int>((begin + t.steps - 1) / run);
+    const int slot0 = begin > w0 * run ? 1 : 0;
+    const float* ml = r.part + 2ll * r.runs * kRows * DIM;
+    for (int i = 32 * blockIdx.y + warp; i < 32 * blockIdx.y + 32; i += 8) {
+        const int row = t.row0 + i;
+        if (row >= t.n * group) break;
+        auto slot = [&](int w) { return (2ll * w + (w == w0 ? slot0 : 0)) * kRows + i; };
+        float m = -INFINITY, l = 0.f, o[kPer];
+        for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, ml[slot(w) * 2]);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) o[c] = 0.f;
+#pragma unroll 4
+        for (int w = w0; w <= w1; ++w) {
+            const float2 x = *reinterpret_cast<const float2*>(ml + slot(w) * 2);
+            const float f = ex2_approx(x.x - ref);
+            l = fmaf(x.y, f, l);
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) o[c] = fmaf(r.part[slot(w) * DIM + 32 * c + lane], f, o[c]);
+        }
+        const int64_t at = static_cast<int64_t>(t.first + row / group) * p.a.q_heads + head * group + row % group;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) from_f32(o[c] * row_inverse(l), static_cast<T*>(p.a.out)[at * DIM + 32 * c + lane]);
+        if (p.a.lse && lane == 0) p.a.lse[at] = row_lse(m, l);
+    }
+}
+
+int64_t tile_count(const AttendParams& p) {
+    return static_cast<int64_t>(p.b.tokens) * (p.a.q_heads / p.c.kv_heads) / kRows + p.b.n_seq;
+}
+int64_t tile_bytes(const AttendParams& p) { return ((tile_count(p) + 1) * static_cast<int64_t>(sizeof(Tile)) + 255) / 256 * 256; }
+
+template <typename T, int DIM>
+int launch(const AttendParams& p, void* workspace, cudaStream_t st) {
+    using C = Cfg<DIM>;
+    static PerDeviceOnce smem_once;
+    const int rc = set_smem_limit_once(smem_once, k_attend_tiles<T, DIM>, C::kSmem, "cudaFuncSetAttribute(k_attend_tiles)");
+    if (rc) return rc;
+    if (tile_count(p) > 0x7ffffffell) return set_error(B3_EINVAL, "b3_kv_attend: too many tokens for one call");
+    TilesParams r{p, static_cast<int>(tile_count(p)), device_sms(), static_cast<Tile*>(workspace),
+                  reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tile_bytes(p))};
+    k_attend_plan<<<1, 1024, 0, st>>>(r);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return set_cuda_error("k_attend_plan", e);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(r.runs);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, k_attend_tiles<T, DIM>, r);
+    if (e != cudaSuccess) return set_cuda_error("k_attend_tiles", e);
+    cfg.gridDim = dim3(r.runs, kRows / 32);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, k_attend_tiles_join<T, DIM>, r);
+    return e == cudaSuccess ? 0 : set_cuda_error("k_attend_tiles_join", e);
+}
+
+}  // namespace
+
+int64_t attend_tiles_workspace(const AttendParams& p) {
+    return tile_bytes(p) + static_cast<int64_t>(device_sms()) * 2 * kRows * (p.c.head_dim + 2) * 4;
+}
+
+int launch_attend_tiles(const AttendParams& p, void* workspace, cudaStream_t st) {
+    if (p.a.dtype == B3_DTYPE_F16)
+        return p.c.head_dim == 128 ? launch<__half, 128>(p, workspace, st) : launch<__half, 64>(p, workspace, st);
+    return p.c.head_dim == 128 ? launch<__nv_bfloat16, 128>(p, workspace, st) : launch<__nv_bfloat16, 64>(p, workspace, st);
+}
+
+}  // namespace b3
