@@ -196,6 +196,10 @@ __device__ __forceinline__ uint32_t h2u(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_constant__ TilesParams r) {
     using C = Cfg<DIM>;
@@ -218,8 +222,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBar + 128);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(k_full(i), kExpWarps);
-            mbar_init(v_full(i), kExpWarps);
+            mbar_init(k_full(i), 8);
+            mbar_init(v_full(i), 8);
             mbar_init(k_empty(i), 1);
             mbar_init(v_empty(i), 1);
             mbar_init(q_full(i), 4);
@@ -305,18 +309,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
         }
     } else if (warp >= kExpWarp0) {
         // ── codes to f16 operands ──
-        // a warp's loads cover four keys x 128 bytes (eight x 64): a lane takes 16 bytes, lanes of
-        // a quarter-warp four pieces of 64 channels of two keys, so that the swizzled 16-byte
-        // stores of each quarter touch every bank once
-        constexpr int kKeysWarp = 512 / DIM;               // keys of one load of a warp
-        constexpr int kPass = kExpWarps * kKeysWarp;       // keys of one load of all warps
-        constexpr int kLoads = (kKeys + kPass - 1) / kPass;   // loads a thread and operand (the last for some warps)
-        const int ew = warp - kExpWarp0;
+        // Tasks of 16 keys of K or V: the eight of a block's K, then of its V, dealt out to the warps in
+        // turn, so 16 keys are one page and one table entry.  A task's loads are two tasks ahead of its
+        // stores.  A load of a warp covers four keys x 128 bytes (eight x 64); a lane takes 16 bytes, the
+        // lanes of a quarter-warp four pieces of 64 channels of two keys, so that the swizzled 16-byte
+        // stores of each quarter touch every bank once.
+        constexpr int kLoads = DIM / 32;                   // loads a thread and task
+        constexpr int kKeysLoad = 16 / kLoads;             // keys of a load
         const int piece = DIM == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;   // 16 channels
         const int sub = DIM == 128 ? ((lane >> 2) & 1) + 2 * (lane >> 4) : lane >> 2;
-        const int row = ew * kKeysWarp + sub;              // + i * kPass
-        uint4 kc[kLoads], vc[kLoads];
-        int any_lo, any_hi;       // keys that some row of the item sees
+        const int tasks = static_cast<int>(min(w.end - w.at, static_cast<int64_t>(1) << 26)) * 16;
+        const uint32_t dst = smem_u32(smem) + (piece >> 2) * C::kHalf + sub * 128;
+        const int c0 = 2 * (piece & 3);
+        int any_lo, any_hi, block = 0;       // keys that some row of the item sees; block of the run the loads are at
         const int32_t* pages;
         auto item = [&]() {
             const SeqSpan sp = {w.t.first, w.t.n, w.t.len};
@@ -326,28 +331,42 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
             seen_keys(p, sp, last / group, x, any_hi);
             pages = p.b.page_table + w.t.seq * p.b.table_stride;
         };
-        auto load = [&](const uint8_t* codes, uint4 (&c)[kLoads], int block) {
+        item();
+        auto fetch = [&](int q, uint4 (&c)[kLoads]) {
+            if ((q >> 4) != block) {
+                ++block;
+                if (w.s0 + 1 < w.s1) {
+                    ++w.s0, ++w.at;   // Walk::next adds what is left
+                } else {
+                    w.next();
+                    item();
+                }
+            }
+            const int key = w.t.key_lo + w.s0 * kKeys + 16 * (q & 7);
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int key = w.t.key_lo + block * kKeys + row + i * kPass;
-                c[i] = make_uint4(0, 0, 0, 0);   // a key that no row sees: 0, whatever its place holds
-                if (row + i * kPass < kKeys && key >= any_lo && key < any_hi) {
-                    int id = __ldg(pages + (key >> log_page));
-                    if (id < 0 || id >= p.c.pages) {
-                        kv_flag(p.c.status, B3_KV_BAD_PAGE);
-                        id = 0;
-                    }
-                    const int64_t line = (static_cast<int64_t>(id) * heads + w.head) * page + (key & (page - 1));
-                    c[i] = __ldg(reinterpret_cast<const uint4*>(codes + line * DIM + 16 * piece));
+            for (int i = 0; i < kLoads; ++i) c[i] = make_uint4(0, 0, 0, 0);   // a key that no row sees: 0, whatever its place holds
+            if (key + 16 > any_lo && key < any_hi) {
+                int id = __ldg(pages + (key >> log_page));
+                if (id < 0 || id >= p.c.pages) {
+                    kv_flag(p.c.status, B3_KV_BAD_PAGE);
+                    id = 0;
+                }
+                const int line = (id * heads + w.head) * page + (key & (page - 1)) + sub;
+                const uint8_t* from = ((q & 8) ? p.c.v : p.c.k) + static_cast<int64_t>(line) * DIM + 16 * piece;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const int k = key + sub + i * kKeysLoad;
+                    if (k >= any_lo && k < any_hi) c[i] = __ldg(reinterpret_cast<const uint4*>(from + i * kKeysLoad * DIM));
                 }
             }
         };
-        auto expand = [&](uint8_t* to, const uint4 (&c)[kLoads]) {
+        auto expand = [&](int q, const uint4 (&c)[kLoads]) {
+            const uint32_t g = q >> 4, st = g & 1, v = (q >> 3) & 1, key = 16 * (q & 7);
+            if (g >= 2) ok = __all_sync(0xffffffffu, mbar_wait(v ? v_empty(st) : k_empty(st), ((g >> 1) - 1) & 1, 0x75));
+            if (!ok) return;
+            const uint32_t to = dst + (v ? C::kV : C::kK) + st * C::kOperand + key * 128;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int key = row + i * kPass;
-                if (key >= kKeys) break;
-                uint8_t* line = to + (piece >> 2) * C::kHalf + key * 128;
                 const uint32_t in[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
                 uint32_t out[8];
 #pragma unroll
@@ -356,39 +375,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                     out[2 * k] = *reinterpret_cast<const uint32_t*>(&a);
                     out[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&b);
                 }
-                const int c0 = 2 * (piece & 3), sw = key & 7;
-                *reinterpret_cast<uint4*>(line + ((c0 ^ sw) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
-                *reinterpret_cast<uint4*>(line + (((c0 + 1) ^ sw) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+                const int sw = (sub + i * kKeysLoad) & 7;
+                sts128(to + i * kKeysLoad * 128 + ((c0 ^ sw) << 4), out[0], out[1], out[2], out[3]);
+                sts128(to + i * kKeysLoad * 128 + (((c0 + 1) ^ sw) << 4), out[4], out[5], out[6], out[7]);
             }
             fence_async_shared();
             __syncwarp();
+            if (lane == 0) mbar_arrive(v ? v_full(st) : k_full(st));
         };
-        uint32_t g = 0;
-        item();
-        load(p.c.k, kc, w.s0);
-        load(p.c.v, vc, w.s0);
-        bool more = true;
-        while (ok && more) {
-            // this block is in registers; the next one (of this item or the next) is loaded behind it
-            const uint32_t st = g & 1;
-            if (g >= 2) ok = __all_sync(0xffffffffu, mbar_wait(k_empty(st), ((g >> 1) - 1) & 1, 0x75));
-            if (!ok) break;
-            expand(smem + C::kK + st * C::kOperand, kc);
-            if (lane == 0) mbar_arrive(k_full(st));
-            const int j = w.s0;
-            if (j + 1 < w.s1) {
-                ++w.s0, ++w.at;   // Walk::next adds what is left
-            } else {
-                more = w.next();
-                if (more) item();
+        uint4 ca[kLoads], cb[kLoads];
+        const int first = warp - kExpWarp0;
+        if (first < tasks) fetch(first, ca);
+        if (first + kExpWarps < tasks) fetch(first + kExpWarps, cb);
+        for (int q = first; q < tasks && ok; q += 2 * kExpWarps) {
+            expand(q, ca);
+            if (ok && q + 2 * kExpWarps < tasks) fetch(q + 2 * kExpWarps, ca);
+            if (ok && q + kExpWarps < tasks) {
+                expand(q + kExpWarps, cb);
+                if (ok && q + 3 * kExpWarps < tasks) fetch(q + 3 * kExpWarps, cb);
             }
-            if (more) load(p.c.k, kc, w.s0);
-            if (g >= 2) ok = __all_sync(0xffffffffu, mbar_wait(v_empty(st), ((g >> 1) - 1) & 1, 0x76));
-            if (!ok) break;
-            expand(smem + C::kV + st * C::kOperand, vc);
-            if (lane == 0) mbar_arrive(v_full(st));
-            if (more) load(p.c.v, vc, w.s0);
-            ++g;
         }
         if (!ok && lane == 0) kv_flag(p.c.status, B3_KV_TIMEOUT);
     } else {
@@ -477,6 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
             scales(s0, ks_next, ve_next);
             float m = -INFINITY, l = 0.f;
             const float qs = qscale;
+            auto factor = [&](float k) { return fminf(fmaxf(qs * k, 1e-37f), 3.4e38f); };   // finite and positive
             for (int j = s0; j < s1; ++j) {
                 ks = ks_next, ve = ve_next;
                 scales(j + 1, ks_next, ve_next);
@@ -486,35 +492,42 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                 tc_fence_after();
                 const int key = t.key_lo + j * kKeys;
                 const bool whole = key >= lo_max && key + kKeys <= hi_min;
+                if (!whole) {   // scores of keys that a row does not see become -inf in TMEM
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t a[32];
+                        tmem_ld_32x32b_x32(ts + 32 * c, a);
+                        tmem_wait_ld();
+                        const int from = row_lo - key - 32 * c, to_ = row_hi - key - 32 * c;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i < from || i >= to_) a[i] = 0xff800000u;
+                        tmem_st_32x32b_x32(ts + 32 * c, a);
+                    }
+                    tmem_wait_st();
+                }
                 // maximum: of the raw products in each 16 keys, then scaled (the factor is positive)
                 float top = -INFINITY;
+                uint32_t a[2][32];
+                tmem_ld_32x32b_x32(ts, a[0]);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t a[32];
-                    tmem_ld_32x32b_x32(ts + 32 * c, a);
                     tmem_wait_ld();
+                    if (c < 3) tmem_ld_32x32b_x32(ts + 32 * (c + 1), a[(c + 1) & 1]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const int at = 2 * c + u;
-                        const float f = fminf(qs * __shfl_sync(0xffffffffu, ks, at), 3.4e38f);
-                        const float e = static_cast<float>(__shfl_sync(0xffffffffu, ve, at));
+                        const float f = factor(__shfl_sync(0xffffffffu, ks, 2 * c + u));
+                        const float e = static_cast<float>(__shfl_sync(0xffffffffu, ve, 2 * c + u));
                         float g0 = -INFINITY, g1 = -INFINITY;
-                        if (whole) {
 #pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                g0 = fmaxf(g0, __uint_as_float(a[16 * u + i]));
-                                g1 = fmaxf(g1, __uint_as_float(a[16 * u + i + 1]));
-                            }
-                        } else {
-                            const int k0 = key + 16 * at;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (k0 + i >= row_lo && k0 + i < row_hi) g0 = fmaxf(g0, __uint_as_float(a[16 * u + i]));
+                        for (int i = 0; i < 16; i += 2) {
+                            g0 = fmaxf(g0, __uint_as_float(a[c & 1][16 * u + i]));
+                            g1 = fmaxf(g1, __uint_as_float(a[c & 1][16 * u + i + 1]));
                         }
-                        g0 = fmaxf(g0, g1);
-                        if (g0 > -INFINITY) top = fmaxf(top, fmaf(g0, f, e));
+                        top = fmaxf(top, fmaf(fmaxf(g0, g1), f, e));
                     }
                 }
+                tmem_ld_32x32b_x32(ts, a[0]);   // again, for the exponentials
                 const bool grow = top > m + kMove || (m == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float m_new = grow ? top : m;
@@ -522,39 +535,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                     m = m_new;
                     l *= corr;
                     if (j > s0) {   // the products so far are done: S was issued after them
-#pragma unroll
-                        for (int c = 0; c < DIM / 32; ++c) {
-                            uint32_t a[32];
-                            tmem_ld_32x32b_x32(to + 32 * c, a);
+#pragma unroll 1
+                        for (int c = 0; c < DIM / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld_32x32b_x16(to + 16 * c, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * corr);
-                            tmem_st_32x32b_x32(to + 32 * c, a);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                            tmem_st_32x32b_x16(to + 16 * c, o);
                         }
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t a[32], b[16];
-                    tmem_ld_32x32b_x32(ts + 32 * c, a);
+                    uint32_t b[16];
                     tmem_wait_ld();
+                    if (c < 3) tmem_ld_32x32b_x32(ts + 32 * (c + 1), a[(c + 1) & 1]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const int at = 2 * c + u;
-                        const float f = fminf(qs * __shfl_sync(0xffffffffu, ks, at), 3.4e38f);
-                        const int ei = __shfl_sync(0xffffffffu, ve, at);
+                        const float f = factor(__shfl_sync(0xffffffffu, ks, 2 * c + u));
+                        const int ei = __shfl_sync(0xffffffffu, ve, 2 * c + u);
                         const float e = static_cast<float>(ei) - ref;
                         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
-                            float2 y = __ffma2_rn(make_float2(__uint_as_float(a[16 * u + i]), __uint_as_float(a[16 * u + i + 1])),
+                            float2 y = __ffma2_rn(make_float2(__uint_as_float(a[c & 1][16 * u + i]),
+                                                              __uint_as_float(a[c & 1][16 * u + i + 1])),
                                                   make_float2(f, f), make_float2(e, e));
-                            if (!whole) {
-                                const int k0 = key + 16 * at + i;
-                                if (k0 < row_lo || k0 >= row_hi) y.x = -INFINITY;
-                                if (k0 + 1 < row_lo || k0 + 1 >= row_hi) y.y = -INFINITY;
-                            }
                             y = make_float2(ex2_approx(y.x), ex2_approx(y.y));
                             sum = __fadd2_rn(sum, y);
                             b[8 * u + (i >> 1)] = h2u(y.x, y.y);
@@ -645,8 +653,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
     }
 }
 
-// Adds up partial results: block (w, y) takes 32 rows of the item that starts
-// in run w and goes on past it.
+// Adds up partial results: block (w, y) takes eight rows, a warp each, of the
+// item that starts in run w and goes on past it.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(256) k_attend_tiles_join(const __grid_constant__ TilesParams r) {
     constexpr int kPer = DIM / 32;
@@ -673,9 +681,9 @@ __global__ void __launch_bounds__(256) k_attend_tiles_join(const __grid_constant
     const int w1 = static_cast<int>((begin + t.steps - 1) / run);
     const int slot0 = begin > w0 * run ? 1 : 0;
     const float* ml = r.part + 2ll * r.runs * kRows * DIM;
-    for (int i = 32 * blockIdx.y + warp; i < 32 * blockIdx.y + 32; i += 8) {
-        const int row = t.row0 + i;
-        if (row >= t.n * group) break;
+    {
+        const int i = 8 * blockIdx.y + warp, row = t.row0 + i;
+        if (row >= t.n * group) return;
         auto slot = [&](int w) { return (2ll * w + (w == w0 ? slot0 : 0)) * kRows + i; };
         float m = -INFINITY, l = 0.f, o[kPer];
         for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, ml[slot(w) * 2]);
@@ -728,7 +736,7 @@ int launch(const AttendParams& p, void* workspace, cudaStream_t st) {
     cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, k_attend_tiles<T, DIM>, r);
     if (e != cudaSuccess) return set_cuda_error("k_attend_tiles", e);
-    cfg.gridDim = dim3(r.runs, kRows / 32);
+    cfg.gridDim = dim3(r.runs, kRows / 8);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, k_attend_tiles_join<T, DIM>, r);
