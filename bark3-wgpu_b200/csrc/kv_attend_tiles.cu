@@ -653,8 +653,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
     }
 }
 
-// Adds up partial results: block (w, y) takes eight rows, a warp each, of the
-// item that starts in run w and goes on past it.
+// Adds up partial results: block (w, y) takes 32 rows, four a warp at once, of
+// the item that starts in run w and goes on past it.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(256) k_attend_tiles_join(const __grid_constant__ TilesParams r) {
     constexpr int kPer = DIM / 32;
@@ -681,29 +681,39 @@ __global__ void __launch_bounds__(256) k_attend_tiles_join(const __grid_constant
     const int w1 = static_cast<int>((begin + t.steps - 1) / run);
     const int slot0 = begin > w0 * run ? 1 : 0;
     const float* ml = r.part + 2ll * r.runs * kRows * DIM;
-    {
-        const int i = 8 * blockIdx.y + warp, row = t.row0 + i;
-        if (row >= t.n * group) return;
-        auto slot = [&](int w) { return (2ll * w + (w == w0 ? slot0 : 0)) * kRows + i; };
-        float m = -INFINITY, l = 0.f, o[kPer];
-        for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, ml[slot(w) * 2]);
+    const int i0 = 32 * blockIdx.y + 4 * warp, row0 = t.row0 + i0, rows = min(4, t.n * group - row0);
+    if (rows <= 0) return;
+    float m[4], l[4], o[4][kPer];
 #pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        const float ref = m == -INFINITY ? 0.f : m;
+    for (int i = 0; i < 4; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
 #pragma unroll
-        for (int c = 0; c < kPer; ++c) o[c] = 0.f;
-#pragma unroll 4
-        for (int w = w0; w <= w1; ++w) {
-            const float2 x = *reinterpret_cast<const float2*>(ml + slot(w) * 2);
-            const float f = ex2_approx(x.x - ref);
-            l = fmaf(x.y, f, l);
+        for (int c = 0; c < kPer; ++c) o[i][c] = 0.f;
+    }
+    // an item is rarely in more than three runs: the reference moves along
+    for (int w = w0; w <= w1; ++w) {
+        const int64_t at = (2ll * w + (w == w0 ? slot0 : 0)) * kRows + i0;
 #pragma unroll
-            for (int c = 0; c < kPer; ++c) o[c] = fmaf(r.part[slot(w) * DIM + 32 * c + lane], f, o[c]);
+        for (int i = 0; i < 4; ++i) {
+            if (i >= rows) break;
+            const float2 x = *reinterpret_cast<const float2*>(ml + (at + i) * 2);
+            const float top = fmaxf(m[i], x.x), ref = top == -INFINITY ? 0.f : top;
+            const float old = ex2_approx(m[i] - ref), f = ex2_approx(x.x - ref);
+            l[i] = fmaf(x.y, f, l[i] * old);
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) o[i][c] = fmaf(r.part[(at + i) * DIM + 32 * c + lane], f, o[i][c] * old);
+            m[i] = top;
         }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (i >= rows) break;
+        const int row = row0 + i;
         const int64_t at = static_cast<int64_t>(t.first + row / group) * p.a.q_heads + head * group + row % group;
 #pragma unroll
-        for (int c = 0; c < kPer; ++c) from_f32(o[c] * row_inverse(l), static_cast<T*>(p.a.out)[at * DIM + 32 * c + lane]);
-        if (p.a.lse && lane == 0) p.a.lse[at] = row_lse(m, l);
+        for (int c = 0; c < kPer; ++c) from_f32(o[i][c] * row_inverse(l[i]), static_cast<T*>(p.a.out)[at * DIM + 32 * c + lane]);
+        if (p.a.lse && lane == 0) p.a.lse[at] = row_lse(m[i], l[i]);
     }
 }
 
@@ -736,7 +746,7 @@ int launch(const AttendParams& p, void* workspace, cudaStream_t st) {
     cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, k_attend_tiles<T, DIM>, r);
     if (e != cudaSuccess) return set_cuda_error("k_attend_tiles", e);
-    cfg.gridDim = dim3(r.runs, kRows / 8);
+    cfg.gridDim = dim3(r.runs, kRows / 32);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, k_attend_tiles_join<T, DIM>, r);
