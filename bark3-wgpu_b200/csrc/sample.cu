@@ -1,154 +1,572 @@
 // sample.cu — b3_sample: the next token of every row of logits by temperature,
 // top-k, top-p and min-p from a given random number.
 //
-//   w_i = exp((l_i - m) / T) as a whole number of 2^-31, W = their exact sum
+//   w_i = exp((l_i - m) / T) as a whole number of 2^-31 (W_i),  sums exact
 // Sums of whole numbers do not depend on their order, so the answer is the
-// same however the row is split over threads.  The kept tokens are a beginning
-// of the order (falling logit, rising index); it is found by a search over the
-// logits' order-preserving bit patterns, eight bits a pass, then over indices
-// among equals.  One block a row.
+// same however a row is split over threads and blocks.  The kept tokens are a
+// beginning of the order (falling logit, rising index); the answer is the
+// first kept token, by index, at which the running sum of W passes u times the
+// total.
+//
+// A row is read once, into the registers of a cluster of 1 to 8 blocks (512
+// threads, EPT values each; a warp's values are neighbours, in index order
+// over (vector, lane, place)).  Bound by memory for many rows, by the chain of
+// block- and cluster-wide steps for few.
+//   top_k <= 512   Each warp's j-th largest thread maximum, j = ceil(k / 16),
+//                  bounds the k-th largest logit from below (16 warps hold k
+//                  values that large); what reaches the bound, a few hundred
+//                  candidates, goes to a list in the first block, which ranks
+//                  it by counting and does the rest alone: no weight of the
+//                  row's bulk is ever computed.
+//   top_p, larger  Weights replace the logits in the registers.  A histogram
+//   top_k          over the leading bits of W (64 bins an octave, so a bell of
+//                  logits spreads over hundreds of bins and shared-memory
+//                  atomics rarely meet) finds the bin where the sum reaches its
+//                  goal; that bin's few members go to the list and are ranked.
+//   long ties      A list that overflows (a thousand equal logits and more)
+//                  falls back to a search over the bits of (logit, index).
+#include <cooperative_groups.h>
+
 #include "kv_cache.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace b3 {
 namespace {
 
+using u32 = uint32_t;
+using u64 = unsigned long long;
+
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMaxBlocks = 8;        // of a cluster: the portable limit
+constexpr int kList = 2048;          // candidates
+constexpr int kBins = 2048;
+constexpr int kTopList = 512;        // top_k up to here ranks candidates: one a thread afterwards
 
-// Order-preserving bits of a logit: larger logits, larger keys; -0 = +0; NaN
-// and -inf give 0 (they weigh nothing and are never taken).
-__device__ __forceinline__ uint32_t key_of(float x) {
-    if (!(x > -INFINITY)) return 0;
-    const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);
+struct Shared {
+    union {
+        struct {
+            u64 key[kList];              // (order of the logit, ~index)
+            u32 weight[kList];           // by rank
+        } list;
+        struct {
+            u32 lo[kBins], hi[kBins];    // sums of W's lower and upper 16 bits (or counts and nothing)
+        } hist;
+    };
+    u64 warp_sum[kWarps];
+    float warp_f[2 * kWarps];
+    // written by the other blocks of the cluster
+    float peak[kMaxBlocks], bound[kMaxBlocks];
+    u64 part[2][kMaxBlocks];
+    u64 cut_before, cut_key;
+    int cut_bin, count, best;
+};
+
+// Order-preserving bits of a logit: larger logits, larger keys; -0 = +0.
+__device__ __forceinline__ u32 key_of(float x) {
+    const u32 b = __float_as_uint(x == 0.f ? 0.f : x);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float logit_of(u32 key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ u64 rank_key(float x, int i) { return static_cast<u64>(key_of(x)) << 32 | static_cast<u32>(~i); }
 
-__device__ __forceinline__ float weight_of(float x, float peak, float t) { return x == peak ? 1.f : expf((x - peak) / t); }
-__device__ __forceinline__ unsigned long long whole(float w) { return static_cast<unsigned long long>(w * 2147483648.f); }
+// exp((x - peak) / t) with the division rounded as IEEE's.  inv = 1 / t
+// correctly rounded: then q = a inv is next to a / t, r = a - q t is exact in
+// one fused multiply-add, and q + r inv is a / t correctly rounded unless t's
+// significand is all ones (P. Markstein, "Computation of elementary functions
+// on the IBM RISC System/6000 processor", 1990); such t, and ones so far out
+// that a residual could leave the normal range, are divided by.
+struct Weigh {
+    float peak, t, inv;
+    bool divide;
+    __device__ __forceinline__ void set(float p, float temperature) {
+        peak = p;
+        t = temperature;
+        inv = __frcp_rn(t);
+        divide = (__float_as_uint(t) & 0x7fffffu) == 0x7fffffu || !(t > 0x1p-60f && t < 0x1p60f);
+    }
+    __device__ __forceinline__ float power(float x) const {
+        const float a = x - peak;
+        if (divide || !(a > -0x1p60f)) return a / t;
+        const float q = a * inv;
+        return fmaf(fmaf(-q, t, a), inv, q);
+    }
+    __device__ __forceinline__ float operator()(float x) const { return x == peak ? 1.f : expf(power(x)); }
+};
+__device__ __forceinline__ u32 whole(float w) { return static_cast<u32>(w * 2147483648.f); }
 
-template <typename V>
-__device__ __forceinline__ V block_sum(V v, V* sh) {
-    for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+// Leading bits of a weight: exponent and six more, 0 .. 2047 for W >= 1.
+__device__ __forceinline__ int bin_of(u32 w) { return static_cast<int>((__float_as_uint(__uint2float_rd(w)) >> 17) - (127u << 6)); }
+
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+// Inclusive sums over the block's threads; `all` their total.
+__device__ __forceinline__ u64 block_scan(u64 v, u64* sums, u64& all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += x;
+    }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    if (lane == 31) sums[warp] = v;
     __syncthreads();
-    V t = 0;
-    for (int w = 0; w < kWarps; ++w) t += sh[w];
-    return t;
+    u64 before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        before += w < warp ? sums[w] : 0;
+        all += sums[w];
+    }
+    return before + v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_sample(const b3_sample_args a) {
-    __shared__ float shf[kWarps];
-    __shared__ unsigned long long shu[kWarps], bin_w[256];
-    __shared__ int found;
-    const int row = blockIdx.x, tid = threadIdx.x, n = a.vocab;
-    const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-    auto at = [&](int i) { return to_f32(x[i]); };
+template <typename T, int EPT>
+struct Row {
+    static constexpr int kVec = 16 / sizeof(T);      // values of a load
+    static constexpr int kLoads = EPT / kVec;
+    const T* x;            // the row
+    int n, off;            // off: values from the 16-byte boundary before the row to its start
+    int base;              // place of this thread's first value
+    bool by_one;           // values one by one: off is 0 wherever the row starts
+    // place of value e: index + off
+    __device__ __forceinline__ int index(int e) const { return base + (e / kVec) * 32 * kVec + e % kVec - off; }
+    __device__ __forceinline__ float at(int i) const { return to_f32(x[i]); }
 
-    uint32_t kmax = 0;
-    for (int i = tid; i < n; i += kThreads) kmax = max(kmax, key_of(at(i)));
-    kmax = __reduce_max_sync(0xffffffffu, kmax);
-    if ((tid & 31) == 0) shf[tid >> 5] = __uint_as_float(kmax);
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w) kmax = max(kmax, __float_as_uint(shf[w]));
-    if (tid == 0) found = n;
-    __syncthreads();
-    if (kmax == 0) {
-        if (tid == 0) {
-            a.ids[row] = -1;
-            if (a.logprob) a.logprob[row] = __uint_as_float(0x7fffffffu);
-        }
-        return;
-    }
-    const float peak = __uint_as_float(kmax & 0x80000000u ? kmax & 0x7fffffffu : ~kmax);
-    const float t = a.temperature ? a.temperature[row] : 1.f;
-    if (!(t > 0.f)) {
-        for (int i = tid; i < n; i += kThreads)
-            if (key_of(at(i)) == kmax) atomicMin(&found, i);
-        __syncthreads();
-        if (tid == 0) {
-            a.ids[row] = found;
-            if (a.logprob) a.logprob[row] = 0.f;
-        }
-        return;
-    }
-    const int top_k = a.top_k ? a.top_k[row] : 0;
-    const float top_p = a.top_p ? a.top_p[row] : 1.f;
-    const float min_p = a.min_p ? a.min_p[row] : 0.f;
-
-    // kept: key > cut, or key == cut and index <= last
-    uint32_t cut = 1;
-    int last = n;
-    for (int stage = 0; stage < 2; ++stage) {
-        if (stage == 0 ? !(top_k > 0 && top_k < n) : !(top_p < 1.f)) continue;
-        unsigned long long sum = 0, goal;   // keep the shortest beginning that reaches `goal`
-        if (stage == 0) {
-            goal = top_k;
-        } else {
-            for (int i = tid; i < n; i += kThreads) {
-                const uint32_t k = key_of(at(i));
-                if (k > cut || (k == cut && i <= last)) sum += whole(weight_of(at(i), peak, t));
+    // the thread's values; what is no number, or outside the row, is -inf
+    __device__ __forceinline__ void load(float (&v)[EPT]) const {
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) {
+            const int i = index(c * kVec);
+            if (i >= 0 && i + kVec <= n && !by_one) {
+                T t[kVec];
+                *reinterpret_cast<uint4*>(t) = __ldcs(reinterpret_cast<const uint4*>(x + i));
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) v[c * kVec + k] = to_f32(t[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kVec; ++k) v[c * kVec + k] = i + k >= 0 && i + k < n ? to_f32(x[i + k]) : -INFINITY;
             }
-            sum = block_sum(sum, shu);
-            const double mass = static_cast<double>(top_p) * static_cast<double>(sum);
-            goal = mass > 0. ? static_cast<unsigned long long>(ceil(mass)) : 1;
         }
-        uint32_t prefix = 0;
-        unsigned long long before = 0;   // weight of the keys above the prefix
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            for (int i = tid; i < 256; i += kThreads) bin_w[i] = 0;
-            __syncthreads();
-            for (int i = tid; i < n; i += kThreads) {
-                const uint32_t k = key_of(at(i));
-                if (k && (shift == 24 || (k >> (shift + 8)) == prefix) && (k > cut || (k == cut && i <= last)))
-                    atomicAdd(&bin_w[(k >> shift) & 255], stage == 0 ? 1ull : whole(weight_of(at(i), peak, t)));
-            }
-            __syncthreads();
-            int b = 255;
-            for (; b > 0 && before + bin_w[b] < goal; --b) before += bin_w[b];
-            prefix = prefix << 8 | b;
-        }
-        // among equals, by index
-        int lo = -1, hi = n - 1;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            sum = 0;
-            for (int i = tid; i <= mid; i += kThreads)
-                if (key_of(at(i)) == prefix) sum += stage == 0 ? 1ull : whole(weight_of(at(i), peak, t));
-            if (before + block_sum(sum, shu) >= goal) hi = mid; else lo = mid;
-        }
-        last = prefix == cut ? min(last, hi) : hi;
-        cut = max(prefix, 1u);
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) v[e] = v[e] > -INFINITY ? v[e] : -INFINITY;
     }
+};
 
-    auto kept = [&](int i) -> unsigned long long {
-        const float v = at(i);
-        const uint32_t k = key_of(v);
-        if (!(k > cut || (k == cut && i <= last))) return 0;
-        const float w = weight_of(v, peak, t);
-        return w >= min_p ? whole(w) : 0;
-    };
-    unsigned long long total = 0;
-    for (int i = tid; i < n; i += kThreads) total += kept(i);
-    total = block_sum(total, shu);
-    // below 0 or no number: the first kept token; 1 and above: the last
-    const double mark = fmin(fmax(static_cast<double>(a.uniform[row]), 0.) * static_cast<double>(total),
-                             static_cast<double>(total) - 1.);
-    int lo = -1, hi = n - 1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        unsigned long long sum = 0;
-        for (int i = tid; i <= mid; i += kThreads) sum += kept(i);
-        if (static_cast<double>(block_sum(sum, shu)) > mark) hi = mid; else lo = mid;
+// Ranks of the list's entries, largest key first: entry i of thread `tid`,
+// tid + 512, ... ; f(rank, key).  Keys differ.
+template <typename F>
+__device__ __forceinline__ void rank_list(const u64* key, int n, F f) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const u64 mine = key[i];
+        int rank = 0;
+        int j = 0;
+        for (; j + 4 <= n; j += 4)
+            rank += (key[j] > mine) + (key[j + 1] > mine) + (key[j + 2] > mine) + (key[j + 3] > mine);
+        for (; j < n; ++j) rank += key[j] > mine;
+        f(rank, mine);
+    }
+}
+
+__device__ __forceinline__ float log_weight(u64 total) { return logf(static_cast<float>(total) * (1.f / 2147483648.f)); }
+
+// u total, so that the first token whose running sum exceeds it is the answer;
+// below 0 or no number: the first kept token, 1 and above: the last.
+__device__ __forceinline__ u64 mark_of(float u, u64 total) {
+    const double all = static_cast<double>(total);
+    return static_cast<u64>(fmin(fmax(static_cast<double>(u), 0.) * all, all - 1.));
+}
+__device__ __forceinline__ u64 mass_goal(float p, u64 total) {   // what the kept beginning has to reach
+    const double mass = static_cast<double>(p) * static_cast<double>(total);
+    return mass > 0. ? static_cast<u64>(ceil(mass)) : 1;
+}
+
+template <typename T, int EPT>
+__global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __grid_constant__ b3_sample_args a, bool by_one) {
+    __shared__ Shared s;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int blocks = cluster.num_blocks(), me = cluster.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / blocks;
+    Shared* const first = cluster.map_shared_rank(&s, 0);
+
+    Row<T, EPT> r;
+    r.x = static_cast<const T*>(a.logits) + row * a.row_stride;
+    r.n = a.vocab;
+    r.by_one = by_one;
+    r.off = by_one ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(r.x) & 15) / sizeof(T));
+    r.base = (me * kWarps + warp) * 32 * EPT + lane * Row<T, EPT>::kVec;
+    float v[EPT];
+    r.load(v);
+    const float t = a.temperature ? __ldg(a.temperature + row) : 1.f;
+    const int top_k = a.top_k ? __ldg(a.top_k + row) : 0;
+    const float top_p = a.top_p ? __ldg(a.top_p + row) : 1.f;
+    const float min_p = a.min_p ? __ldg(a.min_p + row) : 0.f;
+    const float u = __ldg(a.uniform + row);
+    const bool sampled = t > 0.f;
+    const bool by_list = sampled && top_k > 0 && top_k <= kTopList && top_k < r.n;
+
+    // ── the largest logit, and a lower bound of the k-th ──
+    float peak = v[0];
+#pragma unroll
+    for (int e = 1; e < EPT; ++e) peak = fmaxf(peak, v[e]);
+    float jth = -INFINITY;
+    if (by_list) {
+        // bitonic sort of the warp's thread maxima, largest in lane 0
+        float x = peak;
+#pragma unroll
+        for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+            for (int d = k >> 1; d; d >>= 1) {
+                const float y = __shfl_xor_sync(0xffffffffu, x, d);
+                const bool larger = ((lane & d) == 0) == ((lane & k) == 0);
+                x = larger ? fmaxf(x, y) : fminf(x, y);
+            }
+        jth = __shfl_sync(0xffffffffu, x, (top_k + kWarps - 1) / kWarps - 1);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, d));
+    if (lane == 0) {
+        s.warp_f[warp] = peak;
+        s.warp_f[kWarps + warp] = jth;
     }
     if (tid == 0) {
-        a.ids[row] = total ? hi : -1;
-        if (a.logprob)
-            a.logprob[row] = total ? (at(hi) == peak ? 0.f : (at(hi) - peak) / t) - logf(static_cast<float>(total) * (1.f / 2147483648.f))
-                                   : __uint_as_float(0x7fffffffu);
+        s.count = 0;
+        s.best = r.n;
     }
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) {
+        peak = fmaxf(peak, s.warp_f[w]);
+        jth = fminf(jth, s.warp_f[kWarps + w]);
+    }
+    if (blocks > 1) {
+        if (tid < blocks) {
+            Shared* const to = cluster.map_shared_rank(&s, tid);
+            to->peak[me] = peak;
+            to->bound[me] = jth;
+        }
+        cluster.sync();
+        for (int b = 0; b < blocks; ++b) {
+            peak = fmaxf(peak, s.peak[b]);
+            jth = fmaxf(jth, s.bound[b]);
+        }
+    }
+    auto write = [&](int id, float logprob) {
+        a.ids[row] = id;
+        if (a.logprob) a.logprob[row] = logprob;
+    };
+    const float no_number = __uint_as_float(0x7fffffffu);
+    if (!(peak > -INFINITY)) {   // uniform over the cluster, like every choice by the row's settings below
+        if (me == 0 && tid == 0) write(-1, no_number);
+        return;
+    }
+    if (!sampled) {
+        int best = r.n;
+#pragma unroll
+        for (int e = EPT - 1; e >= 0; --e)
+            if (v[e] == peak) best = r.index(e);
+        best = __reduce_min_sync(0xffffffffu, best);
+        if (lane == 0 && best < r.n) atomicMin(&first->best, best);
+        cluster.sync();
+        if (me == 0 && tid == 0) write(s.best, 0.f);
+        return;
+    }
+    Weigh weigh;
+    weigh.set(peak, t);
+
+    // adds an entry to the first block's list
+    auto enlist = [&](float x, int i) {
+        const int at = atomicAdd(&first->count, 1);
+        if (at < kList) first->list.key[at] = rank_key(x, i);
+    };
+
+    // ── small top_k: candidates only ──
+    if (by_list) {
+#pragma unroll
+        for (int e = 0; e < EPT; ++e)
+            if (v[e] >= jth && v[e] > -INFINITY) enlist(v[e], r.index(e));
+        cluster.sync();
+        const int n = first->count;
+        if (n <= kList) {
+            if (blocks > 1) cluster.sync();   // every block has read the count: the others may leave
+            if (me) return;
+            const int k = min(top_k, n);
+            u64 mine = 0;                     // the entry of rank tid
+            // rank_list reads all keys; the ranked ones are written behind a barrier
+            u64 found[kList / kThreads];
+            int where[kList / kThreads], c = 0;
+            rank_list(s.list.key, n, [&](int rank, u64 key) {
+                found[c] = key;
+                where[c++] = rank;
+            });
+            __syncthreads();
+            for (int i = 0; i < c; ++i)
+                if (where[i] < k) s.list.key[where[i]] = found[i];
+            __syncthreads();
+            float w = 0.f;
+            if (tid < k) {
+                mine = s.list.key[tid];
+                w = weigh(logit_of(static_cast<u32>(mine >> 32)));
+            }
+            u32 W = tid < k ? whole(w) : 0;
+            if (top_p < 1.f) {
+                u64 total;
+                const u64 upto = block_scan(W, s.warp_sum, total);
+                if (tid > 0 && upto - W >= mass_goal(top_p, total)) W = 0;
+            }
+            if (!(w >= min_p)) W = 0;
+            __syncthreads();
+            s.list.weight[tid] = W;
+            __syncthreads();
+            u64 total = 0, before = 0;
+            for (int j = 0; j < k; ++j) {
+                const u32 x = s.list.weight[j];
+                total += x;
+                before += static_cast<u32>(s.list.key[j]) > static_cast<u32>(mine) ? x : 0;   // ~index: larger comes first
+            }
+            if (total == 0) {
+                if (tid == 0) write(-1, no_number);
+                return;
+            }
+            const u64 mark = mark_of(u, total);
+            if (W && before <= mark && mark < before + W) {
+                const float x = logit_of(static_cast<u32>(mine >> 32));
+                write(static_cast<int>(~static_cast<u32>(mine)), (x == peak ? 0.f : weigh.power(x)) - log_weight(total));
+            }
+            return;
+        }
+        cluster.sync();
+        if (me == 0 && tid == 0) s.count = 0;
+    }
+
+    // ── weights in place of the logits ──
+    u32 W[EPT];
+    u64 keep = 0;   // min_p lets value e through
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) {
+        const float w = v[e] > -INFINITY ? weigh(v[e]) : 0.f;
+        W[e] = whole(w);
+        keep |= static_cast<u64>(w >= min_p) << e;
+    }
+
+    // ── top_k (by counts), then top_p (by weights): a beginning of the order ──
+    for (int stage = 0; stage < 2; ++stage) {
+        if (stage == 0 ? !(top_k > 0 && top_k < r.n) : !(top_p < 1.f)) continue;
+        __syncthreads();
+        for (int i = tid; i < kBins; i += kThreads) s.hist.lo[i] = s.hist.hi[i] = 0;
+        if (tid == 0) s.cut_bin = -1;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < EPT; ++e)
+            if (W[e]) {
+                const int b = bin_of(W[e]);
+                if (stage == 0) {
+                    atomicAdd(&s.hist.lo[b], 1u);
+                } else {
+                    atomicAdd(&s.hist.lo[b], W[e] & 0xffffu);
+                    if (W[e] >> 16) atomicAdd(&s.hist.hi[b], W[e] >> 16);
+                }
+            }
+        cluster.sync();
+        // each block adds up its share of the bins, the largest weights first, over all blocks
+        const int share = kBins / blocks, per = (share + kThreads - 1) / kThreads;
+        u64 sums[kBins / kThreads], mine = 0;
+        for (int i = 0; i < per; ++i) {
+            const int bin = kBins - 1 - (me * share + tid * per + i);
+            sums[i] = 0;
+            if (tid * per + i < share)
+                for (int b = 0; b < blocks; ++b) {
+                    const Shared* const from = cluster.map_shared_rank(&s, b);
+                    sums[i] += from->hist.lo[bin] + (static_cast<u64>(from->hist.hi[bin]) << 16);
+                }
+            mine += sums[i];
+        }
+        u64 all;
+        u64 upto = block_scan(mine, s.warp_sum, all);
+        if (tid < blocks) cluster.map_shared_rank(&s, tid)->part[0][me] = all;
+        cluster.sync();
+        u64 total = 0, before = 0;
+        for (int b = 0; b < blocks; ++b) {
+            before += b < me ? s.part[0][b] : 0;
+            total += s.part[0][b];
+        }
+        const u64 goal = stage == 0 ? static_cast<u64>(top_k) : mass_goal(top_p, total);
+        if (goal < total || stage == 1) {   // else every weight stays
+            u64 at = before + upto - mine;
+            for (int i = 0; i < per; ++i) {
+                if (at < goal && at + sums[i] >= goal)
+                    for (int b = 0; b < blocks; ++b) {
+                        Shared* const to = cluster.map_shared_rank(&s, b);
+                        to->cut_bin = kBins - 1 - (me * share + tid * per + i);
+                        to->cut_before = at;
+                    }
+                at += sums[i];
+            }
+        }
+        cluster.sync();   // the cut is known, and the histograms (where the list lies) have been read
+        const int cut = s.cut_bin;
+        if (cut < 0) continue;
+        const u64 above = s.cut_before;
+#pragma unroll
+        for (int e = 0; e < EPT; ++e)
+            if (W[e] && bin_of(W[e]) == cut) enlist(r.at(r.index(e)), r.index(e));
+        cluster.sync();
+        const int n = first->count;
+        u64 cut_key;
+        if (n <= kList) {
+            if (me == 0) {
+                u64 found[kList / kThreads];
+                int where[kList / kThreads], c = 0;
+                rank_list(s.list.key, n, [&](int rank, u64 key) {
+                    found[c] = key;
+                    where[c++] = rank;
+                });
+                __syncthreads();
+                for (int i = 0; i < c; ++i) {
+                    s.list.key[where[i]] = found[i];
+                    s.list.weight[where[i]] = stage == 0 ? 1u : whole(weigh(logit_of(static_cast<u32>(found[i] >> 32))));
+                }
+                __syncthreads();
+                constexpr int kPer = kList / kThreads;
+                u64 own = 0, sum;
+                for (int i = 0; i < kPer; ++i) own += kPer * tid + i < n ? s.list.weight[kPer * tid + i] : 0;
+                u64 at_ = above + block_scan(own, s.warp_sum, sum) - own;
+                for (int i = 0; i < kPer && kPer * tid + i < n; ++i) {
+                    const u32 x = s.list.weight[kPer * tid + i];
+                    if (at_ < goal && at_ + x >= goal)   // the last that stays
+                        for (int b = 0; b < blocks; ++b) cluster.map_shared_rank(&s, b)->cut_key = s.list.key[kPer * tid + i];
+                    at_ += x;
+                }
+            }
+            cluster.sync();
+            cut_key = s.cut_key;
+        } else {
+            // bit by bit, the largest key whose entries and those above it reach the goal
+            cut_key = 0;
+            for (int bit = 63, turn = 0; bit >= 0; --bit, turn ^= 1) {
+                const u64 want = cut_key | 1ull << bit;
+                u64 own = 0;
+#pragma unroll
+                for (int e = 0; e < EPT; ++e)
+                    if (W[e] && bin_of(W[e]) == cut && rank_key(r.at(r.index(e)), r.index(e)) >= want) own += stage == 0 ? 1 : W[e];
+                u64 sum;
+                block_scan(own, s.warp_sum, sum);
+                if (tid < blocks) cluster.map_shared_rank(&s, tid)->part[turn][me] = sum;
+                cluster.sync();
+                sum = above;
+                for (int b = 0; b < blocks; ++b) sum += s.part[turn][b];
+                if (sum >= goal) cut_key = want;
+            }
+            cluster.sync();
+        }
+        if (me == 0 && tid == 0) s.count = 0;
+#pragma unroll
+        for (int e = 0; e < EPT; ++e)
+            if (W[e]) {
+                const int b = bin_of(W[e]);
+                if (b < cut || (b == cut && rank_key(r.at(r.index(e)), r.index(e)) < cut_key)) W[e] = 0;
+            }
+        cluster.sync();
+    }
+
+    // ── the token ──
+#pragma unroll
+    for (int e = 0; e < EPT; ++e)
+        if (!(keep >> e & 1)) W[e] = 0;
+    u64 mine = 0;
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) mine += W[e];
+    mine = warp_sum(mine);
+    __syncthreads();
+    if (lane == 0) s.warp_sum[warp] = mine;
+    __syncthreads();
+    u64 total = 0, before = 0;
+    for (int w = 0; w < kWarps; ++w) {
+        before += w < warp ? s.warp_sum[w] : 0;
+        total += s.warp_sum[w];
+    }
+    if (blocks > 1) {
+        if (tid < blocks) cluster.map_shared_rank(&s, tid)->part[1][me] = total;
+        cluster.sync();
+        total = 0;
+        for (int b = 0; b < blocks; ++b) {
+            before += b < me ? s.part[1][b] : 0;
+            total += s.part[1][b];
+        }
+    }
+    if (total == 0) {
+        if (me == 0 && tid == 0) write(-1, no_number);
+        return;
+    }
+    const u64 mark = mark_of(u, total);
+    if (mark < before || mark >= before + mine) return;
+    // this warp has it: its values in index order are (vector, lane, place)
+    constexpr int kVec = Row<T, EPT>::kVec;
+#pragma unroll
+    for (int c = 0; c < EPT / kVec; ++c) {
+        u64 own = 0;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) own += W[c * kVec + k];
+        u64 upto = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const u64 x = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += x;
+        }
+        u64 at = before + upto - own;
+        if (own && at <= mark && mark < at + own) {
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) {
+                if (at <= mark && mark < at + W[c * kVec + k]) {
+                    const int i = r.index(c * kVec + k);
+                    const float x = r.at(i);
+                    write(i, (x == peak ? 0.f : weigh.power(x)) - log_weight(total));
+                }
+                at += W[c * kVec + k];
+            }
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+}
+
+template <typename T, int EPT>
+int launch(const b3_sample_args& a, int blocks, bool by_one, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * blocks);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {static_cast<unsigned>(blocks), 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_sample<T, EPT>, a, by_one);
+    return e == cudaSuccess ? 0 : set_cuda_error("k_sample", e);
+}
+
+// Values a thread and blocks a row.  Few rows: short chains on more SMs.  Many
+// rows: few blocks each, so that more of a row's steps stay inside a block.
+template <typename T>
+int launch_type(const b3_sample_args& a, cudaStream_t st) {
+    // a row that starts within a 16-byte vector takes up to a vector more places
+    const int vec = 16 / static_cast<int>(sizeof(T));
+    const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.row_stride % vec == 0;
+    const int places = a.vocab + (aligned ? 0 : vec - 1);
+    auto need = [&](int ept, int n) {
+        int b = 1;
+        while (b * kThreads * ept < n) b *= 2;
+        return b;
+    };
+    if (static_cast<int64_t>(a.rows) * kMaxBlocks > 0x7fffffff) return set_error(B3_EINVAL, "%d rows are too many for one call", a.rows);
+    const int sms = device_sms();
+    if (need(8, places) <= kMaxBlocks && static_cast<int64_t>(a.rows) * need(8, places) <= 2 * sms)
+        return launch<T, 8>(a, need(8, places), false, st);
+    if (need(32, places) <= kMaxBlocks) return launch<T, 32>(a, need(32, places), false, st);
+    if (need(64, places) <= kMaxBlocks) return launch<T, 64>(a, need(64, places), false, st);
+    return launch<T, 64>(a, need(64, a.vocab), true, st);   // the largest vocabulary in unaligned rows
 }
 
 }  // namespace
@@ -166,11 +584,9 @@ extern "C" int b3_sample(const b3_sample_args* args, void* stream) {
                          B3_SAMPLE_MAX_VOCAB, static_cast<long long>(a.row_stride));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (a.dtype) {
-        case B3_DTYPE_F32: k_sample<float><<<a.rows, kThreads, 0, st>>>(a); break;
-        case B3_DTYPE_F16: k_sample<__half><<<a.rows, kThreads, 0, st>>>(a); break;
-        case B3_DTYPE_BF16: k_sample<__nv_bfloat16><<<a.rows, kThreads, 0, st>>>(a); break;
+        case B3_DTYPE_F32: return launch_type<float>(a, st);
+        case B3_DTYPE_F16: return launch_type<__half>(a, st);
+        case B3_DTYPE_BF16: return launch_type<__nv_bfloat16>(a, st);
         default: return set_error(B3_EINVAL, "dtype %d", a.dtype);
     }
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? 0 : set_cuda_error("k_sample", e);
 }
