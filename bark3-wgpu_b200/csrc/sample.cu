@@ -8,17 +8,20 @@
 // first kept token, by index, at which the running sum of W passes u times the
 // total.
 //
-// A row is read once, into the registers of a cluster of 1 to 8 blocks (512
-// threads, EPT values each; a warp's values are neighbours, in index order
-// over (vector, lane, place)).  Bound by memory for many rows, by the chain of
-// block- and cluster-wide steps for few.
+// A row is read once, into the shared memory of a cluster of 1 to 8 blocks of
+// 512 threads (a column of values for each thread, touched by it alone; a
+// warp's values are neighbours in the row, in index order over (vector, lane,
+// place)).  Shared memory and not registers: loops over 32 values unrolled
+// with an exponential in each miss the instruction cache (204 against ?? us for
+// 256 rows x 131072).  Bound by the instructions of some twenty operations a
+// value for many rows, by the chain of block- and cluster-wide steps for few.
 //   top_k <= 512   Each warp's j-th largest thread maximum, j = ceil(k / 16),
 //                  bounds the k-th largest logit from below (16 warps hold k
 //                  values that large); what reaches the bound, a few hundred
 //                  candidates, goes to a list in the first block, which ranks
 //                  it by counting and does the rest alone: no weight of the
 //                  row's bulk is ever computed.
-//   top_p, larger  Weights replace the logits in the registers.  A histogram
+//   top_p, larger  Weights replace the logits.  A histogram
 //   top_k          over the leading bits of W (64 bins an octave, so a bell of
 //                  logits spreads over hundreds of bins and shared-memory
 //                  atomics rarely meet) finds the bin where the sum reaches its
@@ -125,35 +128,49 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* sums, u64& all) {
     return before + v;
 }
 
-template <typename T, int EPT>
+template <typename T>
 struct Row {
     static constexpr int kVec = 16 / sizeof(T);      // values of a load
-    static constexpr int kLoads = EPT / kVec;
     const T* x;            // the row
     int n, off;            // off: values from the 16-byte boundary before the row to its start
     int base;              // place of this thread's first value
+    int count;             // values a thread, a multiple of kVec
     bool by_one;           // values one by one: off is 0 wherever the row starts
     // place of value e: index + off
     __device__ __forceinline__ int index(int e) const { return base + (e / kVec) * 32 * kVec + e % kVec - off; }
     __device__ __forceinline__ float at(int i) const { return to_f32(x[i]); }
 
-    // the thread's values; what is no number, or outside the row, is -inf
-    __device__ __forceinline__ void load(float (&v)[EPT]) const {
+    // The thread's values into its column, their maximum; what is no number, or outside the row, is -inf.
+    __device__ __forceinline__ float load(float* col) const {
+        float top = -INFINITY;
+        constexpr int kAhead = 4;      // vectors in flight
+        for (int c0 = 0; c0 < count; c0 += kAhead * kVec) {
+            uint4 raw[kAhead];
 #pragma unroll
-        for (int c = 0; c < kLoads; ++c) {
-            const int i = index(c * kVec);
-            if (i >= 0 && i + kVec <= n && !by_one) {
-                T t[kVec];
-                *reinterpret_cast<uint4*>(t) = __ldcs(reinterpret_cast<const uint4*>(x + i));
+            for (int c = 0; c < kAhead; ++c) {
+                const int e = c0 + c * kVec, i = index(e);
+                if (e < count && i >= 0 && i + kVec <= n && !by_one) raw[c] = __ldcs(reinterpret_cast<const uint4*>(x + i));
+            }
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) v[c * kVec + k] = to_f32(t[k]);
-            } else {
+            for (int c = 0; c < kAhead; ++c) {
+                const int e = c0 + c * kVec, i = index(e);
+                if (e >= count) break;
+                const bool vector = i >= 0 && i + kVec <= n && !by_one;
+                const T* t = reinterpret_cast<const T*>(&raw[c]);
 #pragma unroll
-                for (int k = 0; k < kVec; ++k) v[c * kVec + k] = i + k >= 0 && i + k < n ? to_f32(x[i + k]) : -INFINITY;
+                for (int k = 0; k < kVec; ++k) {
+                    float y = -INFINITY;
+                    if (vector)
+                        y = to_f32(t[k]);
+                    else if (i + k >= 0 && i + k < n)
+                        y = to_f32(x[i + k]);
+                    y = y > -INFINITY ? y : -INFINITY;
+                    top = fmaxf(top, y);
+                    col[(e + k) * kThreads] = y;
+                }
             }
         }
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) v[e] = v[e] > -INFINITY ? v[e] : -INFINITY;
+        return top;
     }
 };
 
@@ -185,22 +202,25 @@ __device__ __forceinline__ u64 mass_goal(float p, u64 total) {   // what the kep
     return mass > 0. ? static_cast<u64>(ceil(mass)) : 1;
 }
 
-template <typename T, int EPT>
-__global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __grid_constant__ b3_sample_args a, bool by_one) {
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ b3_sample_args a, int count, bool by_one) {
+    extern __shared__ float values[];
     __shared__ Shared s;
     const cg::cluster_group cluster = cg::this_cluster();
     const int blocks = cluster.num_blocks(), me = cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / blocks;
     Shared* const first = cluster.map_shared_rank(&s, 0);
+    float* const v = values + tid;                       // value e at v[e * kThreads], its weight then at W
+    u32* const W = reinterpret_cast<u32*>(values) + tid;
 
-    Row<T, EPT> r;
+    Row<T> r;
     r.x = static_cast<const T*>(a.logits) + row * a.row_stride;
     r.n = a.vocab;
     r.by_one = by_one;
     r.off = by_one ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(r.x) & 15) / sizeof(T));
-    r.base = (me * kWarps + warp) * 32 * EPT + lane * Row<T, EPT>::kVec;
-    float v[EPT];
-    r.load(v);
+    r.count = count;
+    r.base = (me * kWarps + warp) * 32 * count + lane * Row<T>::kVec;
+    float peak = r.load(v);
     const float t = a.temperature ? __ldg(a.temperature + row) : 1.f;
     const int top_k = a.top_k ? __ldg(a.top_k + row) : 0;
     const float top_p = a.top_p ? __ldg(a.top_p + row) : 1.f;
@@ -210,9 +230,6 @@ __global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __
     const bool by_list = sampled && top_k > 0 && top_k <= kTopList && top_k < r.n;
 
     // ── the largest logit, and a lower bound of the k-th ──
-    float peak = v[0];
-#pragma unroll
-    for (int e = 1; e < EPT; ++e) peak = fmaxf(peak, v[e]);
     float jth = -INFINITY;
     if (by_list) {
         // bitonic sort of the warp's thread maxima, largest in lane 0
@@ -265,9 +282,8 @@ __global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __
     }
     if (!sampled) {
         int best = r.n;
-#pragma unroll
-        for (int e = EPT - 1; e >= 0; --e)
-            if (v[e] == peak) best = r.index(e);
+        for (int e = count - 1; e >= 0; --e)
+            if (v[e * kThreads] == peak) best = r.index(e);
         best = __reduce_min_sync(0xffffffffu, best);
         if (lane == 0 && best < r.n) atomicMin(&first->best, best);
         cluster.sync();
@@ -285,9 +301,11 @@ __global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __
 
     // ── small top_k: candidates only ──
     if (by_list) {
-#pragma unroll
-        for (int e = 0; e < EPT; ++e)
-            if (v[e] >= jth && v[e] > -INFINITY) enlist(v[e], r.index(e));
+#pragma unroll 8
+        for (int e = 0; e < count; ++e) {
+            const float x = v[e * kThreads];
+            if (x >= jth && x > -INFINITY) enlist(x, r.index(e));
+        }
         cluster.sync();
         const int n = first->count;
         if (n <= kList) {
@@ -343,12 +361,11 @@ __global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __
     }
 
     // ── weights in place of the logits ──
-    u32 W[EPT];
     u64 keep = 0;   // min_p lets value e through
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-        const float w = v[e] > -INFINITY ? weigh(v[e]) : 0.f;
-        W[e] = whole(w);
+#pragma unroll 4
+    for (int e = 0; e < count; ++e) {
+        const float x = v[e * kThreads], w = x > -INFINITY ? weigh(x) : 0.f;
+        W[e * kThreads] = whole(w);
         keep |= static_cast<u64>(w >= min_p) << e;
     }
 
@@ -359,17 +376,15 @@ __global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __
         for (int i = tid; i < kBins; i += kThreads) s.hist.lo[i] = s.hist.hi[i] = 0;
         if (tid == 0) s.cut_bin = -1;
         __syncthreads();
-#pragma unroll
-        for (int e = 0; e < EPT; ++e)
-            if (W[e]) {
-                const int b = bin_of(W[e]);
-                if (stage == 0) {
-                    atomicAdd(&s.hist.lo[b], 1u);
-                } else {
-                    atomicAdd(&s.hist.lo[b], W[e] & 0xffffu);
-                    if (W[e] >> 16) atomicAdd(&s.hist.hi[b], W[e] >> 16);
-                }
+#pragma unroll 4
+        for (int e = 0; e < count; ++e) {
+            const u32 x = W[e * kThreads];
+            if (x) {
+                const int b = bin_of(x);
+                atomicAdd(&s.hist.lo[b], stage == 0 ? 1u : x & 0xffffu);
+                if (stage == 1 && x >> 16) atomicAdd(&s.hist.hi[b], x >> 16);
             }
+        }
         cluster.sync();
         // each block adds up its share of the bins, the largest weights first, over all blocks
         const int share = kBins / blocks, per = (share + kThreads - 1) / kThreads;
@@ -410,9 +425,11 @@ __global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __
         const int cut = s.cut_bin;
         if (cut < 0) continue;
         const u64 above = s.cut_before;
-#pragma unroll
-        for (int e = 0; e < EPT; ++e)
-            if (W[e] && bin_of(W[e]) == cut) enlist(r.at(r.index(e)), r.index(e));
+#pragma unroll 4
+        for (int e = 0; e < count; ++e) {
+            const u32 x = W[e * kThreads];
+            if (x && bin_of(x) == cut) enlist(r.at(r.index(e)), r.index(e));
+        }
         cluster.sync();
         const int n = first->count;
         u64 cut_key;
@@ -449,9 +466,10 @@ __global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __
             for (int bit = 63, turn = 0; bit >= 0; --bit, turn ^= 1) {
                 const u64 want = cut_key | 1ull << bit;
                 u64 own = 0;
-#pragma unroll
-                for (int e = 0; e < EPT; ++e)
-                    if (W[e] && bin_of(W[e]) == cut && rank_key(r.at(r.index(e)), r.index(e)) >= want) own += stage == 0 ? 1 : W[e];
+                for (int e = 0; e < count; ++e) {
+                    const u32 x = W[e * kThreads];
+                    if (x && bin_of(x) == cut && rank_key(r.at(r.index(e)), r.index(e)) >= want) own += stage == 0 ? 1 : x;
+                }
                 u64 sum;
                 block_scan(own, s.warp_sum, sum);
                 if (tid < blocks) cluster.map_shared_rank(&s, tid)->part[turn][me] = sum;
@@ -463,22 +481,24 @@ __global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __
             cluster.sync();
         }
         if (me == 0 && tid == 0) s.count = 0;
-#pragma unroll
-        for (int e = 0; e < EPT; ++e)
-            if (W[e]) {
-                const int b = bin_of(W[e]);
-                if (b < cut || (b == cut && rank_key(r.at(r.index(e)), r.index(e)) < cut_key)) W[e] = 0;
+#pragma unroll 4
+        for (int e = 0; e < count; ++e) {
+            const u32 x = W[e * kThreads];
+            if (x) {
+                const int b = bin_of(x);
+                if (b < cut || (b == cut && rank_key(r.at(r.index(e)), r.index(e)) < cut_key)) W[e * kThreads] = 0;
             }
+        }
         cluster.sync();
     }
 
     // ── the token ──
-#pragma unroll
-    for (int e = 0; e < EPT; ++e)
-        if (!(keep >> e & 1)) W[e] = 0;
     u64 mine = 0;
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) mine += W[e];
+    if (min_p > 0.f)
+        for (int e = 0; e < count; ++e)
+            if (!(keep >> e & 1)) W[e * kThreads] = 0;
+#pragma unroll 8
+    for (int e = 0; e < count; ++e) mine += W[e * kThreads];
     mine = warp_sum(mine);
     __syncthreads();
     if (lane == 0) s.warp_sum[warp] = mine;
@@ -504,12 +524,11 @@ __global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __
     const u64 mark = mark_of(u, total);
     if (mark < before || mark >= before + mine) return;
     // this warp has it: its values in index order are (vector, lane, place)
-    constexpr int kVec = Row<T, EPT>::kVec;
-#pragma unroll
-    for (int c = 0; c < EPT / kVec; ++c) {
+    constexpr int kVec = Row<T>::kVec;
+    for (int e = 0; e < count; e += kVec) {
         u64 own = 0;
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) own += W[c * kVec + k];
+        for (int k = 0; k < kVec; ++k) own += W[(e + k) * kThreads];
         u64 upto = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -518,55 +537,60 @@ __global__ void __launch_bounds__(kThreads, EPT <= 32 ? 2 : 1) k_sample(const __
         }
         u64 at = before + upto - own;
         if (own && at <= mark && mark < at + own) {
-#pragma unroll
             for (int k = 0; k < kVec; ++k) {
-                if (at <= mark && mark < at + W[c * kVec + k]) {
-                    const int i = r.index(c * kVec + k);
+                const u32 y = W[(e + k) * kThreads];
+                if (at <= mark && mark < at + y) {
+                    const int i = r.index(e + k);
                     const float x = r.at(i);
                     write(i, (x == peak ? 0.f : weigh.power(x)) - log_weight(total));
                 }
-                at += W[c * kVec + k];
+                at += y;
             }
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
 }
 
-template <typename T, int EPT>
-int launch(const b3_sample_args& a, int blocks, bool by_one, cudaStream_t st) {
+// Values a thread: at most 32 where the row fits a cluster so, else 64 (one
+// block an SM).
+constexpr int kMostValues = 64;
+
+template <typename T>
+int launch(const b3_sample_args& a, cudaStream_t st) {
+    constexpr int kVec = Row<T>::kVec;
+    static PerDeviceOnce smem_once;
+    const int rc = set_smem_limit_once(smem_once, k_sample<T>, kMostValues * kThreads * 4, "cudaFuncSetAttribute(k_sample)");
+    if (rc) return rc;
+    if (static_cast<int64_t>(a.rows) * kMaxBlocks > 0x7fffffff) return set_error(B3_EINVAL, "%d rows are too many for one call", a.rows);
+    // a row that starts within a 16-byte vector takes up to a vector more places
+    const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.row_stride % kVec == 0;
+    bool by_one = false;
+    int places = a.vocab + (aligned ? 0 : kVec - 1);
+    if (places > kMaxBlocks * kThreads * kMostValues) {
+        by_one = true;   // the largest vocabulary in unaligned rows
+        places = a.vocab;
+    }
+    auto values = [&](int blocks) {
+        const int per = kThreads * kVec * blocks;
+        return (places + per - 1) / per * kVec;
+    };
+    // few rows: short columns on more SMs; many: few blocks a row, so that a row's steps stay inside a block
+    int blocks = 1;
+    while (blocks < kMaxBlocks && (values(blocks) > 32 || (values(blocks) > 8 && 2 * blocks * static_cast<int64_t>(a.rows) <= device_sms())))
+        blocks *= 2;
+    const int count = values(blocks);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * blocks);
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(count) * kThreads * 4;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {static_cast<unsigned>(blocks), 1, 1};
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_sample<T, EPT>, a, by_one);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_sample<T>, a, count, by_one);
     return e == cudaSuccess ? 0 : set_cuda_error("k_sample", e);
-}
-
-// Values a thread and blocks a row.  Few rows: short chains on more SMs.  Many
-// rows: few blocks each, so that more of a row's steps stay inside a block.
-template <typename T>
-int launch_type(const b3_sample_args& a, cudaStream_t st) {
-    // a row that starts within a 16-byte vector takes up to a vector more places
-    const int vec = 16 / static_cast<int>(sizeof(T));
-    const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.row_stride % vec == 0;
-    const int places = a.vocab + (aligned ? 0 : vec - 1);
-    auto need = [&](int ept, int n) {
-        int b = 1;
-        while (b * kThreads * ept < n) b *= 2;
-        return b;
-    };
-    if (static_cast<int64_t>(a.rows) * kMaxBlocks > 0x7fffffff) return set_error(B3_EINVAL, "%d rows are too many for one call", a.rows);
-    const int sms = device_sms();
-    if (need(8, places) <= kMaxBlocks && static_cast<int64_t>(a.rows) * need(8, places) <= 2 * sms)
-        return launch<T, 8>(a, need(8, places), false, st);
-    if (need(32, places) <= kMaxBlocks) return launch<T, 32>(a, need(32, places), false, st);
-    if (need(64, places) <= kMaxBlocks) return launch<T, 64>(a, need(64, places), false, st);
-    return launch<T, 64>(a, need(64, a.vocab), true, st);   // the largest vocabulary in unaligned rows
 }
 
 }  // namespace
@@ -584,9 +608,9 @@ extern "C" int b3_sample(const b3_sample_args* args, void* stream) {
                          B3_SAMPLE_MAX_VOCAB, static_cast<long long>(a.row_stride));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (a.dtype) {
-        case B3_DTYPE_F32: return launch_type<float>(a, st);
-        case B3_DTYPE_F16: return launch_type<__half>(a, st);
-        case B3_DTYPE_BF16: return launch_type<__nv_bfloat16>(a, st);
+        case B3_DTYPE_F32: return launch<float>(a, st);
+        case B3_DTYPE_F16: return launch<__half>(a, st);
+        case B3_DTYPE_BF16: return launch<__nv_bfloat16>(a, st);
         default: return set_error(B3_EINVAL, "dtype %d", a.dtype);
     }
 }
