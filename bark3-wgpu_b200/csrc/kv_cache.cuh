@@ -96,6 +96,7 @@ __device__ __forceinline__ void decode8(uint2 c, float (&x)[8]) {
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void from_f32(float x, float& y) { y = x; }
 __device__ __forceinline__ void from_f32(float x, __half& y) { y = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
 
