@@ -55,8 +55,8 @@ _lib = None
 
 
 def build(force: bool = False) -> pathlib.Path:
-    """Compile libbark3_b200.so in place with nvcc (sm_100a)."""
-    if force or not LIB_PATH.exists():
+    """Compile libbark3_b200.so (nvcc, sm_100a) and the torch side of text generation in place."""
+    if force or not LIB_PATH.exists() or not (PKG_DIR / "_textgen.so").exists():
         subprocess.run(["make", "-C", str(PKG_DIR), "-j8"], check=True)
     return LIB_PATH
 
