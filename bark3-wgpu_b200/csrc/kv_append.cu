@@ -12,8 +12,10 @@
 // exponent over all its new rows before it writes a code, so no atomics and no
 // second pass over memory order the scale.  The other blocks own q, a few
 // heads of a token for each warp.  A row of head_dim channels is held by
-// head_dim / 8 lanes, eight channels each: 16-byte loads of 16-bit types, the
-// norm and the rotation's partner channels by shuffles within the row.
+// head_dim / 8 lanes, eight channels each; the norm's sum by shuffles within
+// the row.  PAIRED (the usual rotation of all channels, i with i + head_dim / 2)
+// gives a lane four channels and their four partners, so the rotation stays in
+// the lane; otherwise a lane has eight neighbours and shuffles for partners.
 //   GROUP = 1: a warp a (page, head).  Decode brings one row to each page.
 //   GROUP = 8: a whole block, the page's rows in registers between the
 //              exponent and the codes.  Prompts fill whole pages.
@@ -35,37 +37,137 @@ struct AppendParams {
     int units;
     int kv_blocks;
     int q_chunks;        // warps a token of q
+    int angles16;        // cos and sin are 16-byte aligned
 };
 
-// Norm and rotation of one row piece: channels [8 l, 8 l + 8) of a row whose
-// lanes are consecutive; every lane of the warp takes part.
-template <int DIM>
-__device__ __forceinline__ void turn_row(float (&x)[8], int l, const float* norm, int pos, const b3_kv_append_args& a) {
-    if (norm) {
-        float ss = 0.f;
+// A lane's eight channels of a row: PAIRED [4 l, 4 l + 4) and the same plus
+// DIM / 2, else [8 l, 8 l + 8).
+template <int DIM, bool PAIRED>
+struct Piece {
+    static __device__ __forceinline__ int low(int l) { return PAIRED ? 4 * l : 8 * l; }
+    static __device__ __forceinline__ int high(int l) { return PAIRED ? DIM / 2 + 4 * l : 8 * l + 4; }
+
+    template <bool VEC, typename T>
+    static __device__ __forceinline__ void load(const T* row, int l, float2 (&x)[4]) {
+        T v[8];
+        if (VEC && !PAIRED) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+                reinterpret_cast<uint4*>(v)[i] = __ldcs(reinterpret_cast<const uint4*>(row + 8 * l) + i);
+        } else if (VEC) {
+            if (sizeof(T) == 4) {
+                reinterpret_cast<uint4*>(v)[0] = __ldcs(reinterpret_cast<const uint4*>(row + low(l)));
+                reinterpret_cast<uint4*>(v)[sizeof(T) / 4] = __ldcs(reinterpret_cast<const uint4*>(row + high(l)));
+            } else {
+                reinterpret_cast<uint2*>(v)[0] = __ldcs(reinterpret_cast<const uint2*>(row + low(l)));
+                reinterpret_cast<uint2*>(v)[1] = __ldcs(reinterpret_cast<const uint2*>(row + high(l)));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = row[low(l) + i];
+                v[4 + i] = row[high(l) + i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = make_float2(to_f32(v[2 * i]), to_f32(v[2 * i + 1]));
+    }
+    template <typename T>   // T of 16 bits, row 16-byte aligned
+    static __device__ __forceinline__ void store(T* row, int l, const float2 (&x)[4]) {
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            from_f32(x[i].x, v[2 * i]);
+            from_f32(x[i].y, v[2 * i + 1]);
+        }
+        if (PAIRED) {
+            *reinterpret_cast<uint2*>(row + low(l)) = reinterpret_cast<uint2*>(v)[0];
+            *reinterpret_cast<uint2*>(row + high(l)) = reinterpret_cast<uint2*>(v)[1];
+        } else {
+            *reinterpret_cast<uint4*>(row + 8 * l) = *reinterpret_cast<uint4*>(v);
+        }
+    }
+    static __device__ __forceinline__ void store_codes(uint8_t* row, int l, const float2 (&x)[4], float inv) {
+        const float y[8] = {x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
+        const uint2 c = encode8(y, inv);
+        if (PAIRED) {
+            *reinterpret_cast<uint32_t*>(row + low(l)) = c.x;
+            *reinterpret_cast<uint32_t*>(row + high(l)) = c.y;
+        } else {
+            *reinterpret_cast<uint2*>(row + 8 * l) = c;
+        }
+    }
+    static __device__ __forceinline__ void load_norm(float2 (&w)[4], const float* norm, int l) {
+        if (!norm) return;
+        const float4 a = __ldg(reinterpret_cast<const float4*>(norm + low(l))), b = __ldg(reinterpret_cast<const float4*>(norm + high(l)));
+        w[0] = make_float2(a.x, a.y), w[1] = make_float2(a.z, a.w), w[2] = make_float2(b.x, b.y), w[3] = make_float2(b.z, b.w);
+    }
+};
+
+// A lane's cosines and sines: of its four pairs (PAIRED, interleaved) or of its
+// eight channels (half-split with partners in other lanes).
+struct Angles {
+    float2 c[4], s[4];
+};
+template <int DIM, bool PAIRED>
+__device__ __forceinline__ void load_angles(Angles& g, int l, int pos, const AppendParams& p) {
+    const b3_kv_append_args& a = p.a;
+    const int half = a.rot_dim >> 1, ch = Piece<DIM, PAIRED>::low(l);
+    if (!a.cos || ch >= a.rot_dim) return;
+    const bool four = PAIRED || a.interleaved;
+    const int64_t at = static_cast<int64_t>(pos) * half + (PAIRED ? ch : a.interleaved ? ch >> 1 : ch < half ? ch : ch - half);
+    const float *c = a.cos + at, *s = a.sin + at;
+    if (p.angles16) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (i && four) break;
+            const float4 u = __ldg(reinterpret_cast<const float4*>(c) + i), v = __ldg(reinterpret_cast<const float4*>(s) + i);
+            g.c[2 * i] = make_float2(u.x, u.y), g.c[2 * i + 1] = make_float2(u.z, u.w);
+            g.s[2 * i] = make_float2(v.x, v.y), g.s[2 * i + 1] = make_float2(v.z, v.w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i > 1 && four) break;
+            g.c[i] = make_float2(__ldg(c + 2 * i), __ldg(c + 2 * i + 1));
+            g.s[i] = make_float2(__ldg(s + 2 * i), __ldg(s + 2 * i + 1));
+        }
+    }
+}
+
+__device__ __forceinline__ float2 neg2(float2 x) { return make_float2(-x.x, -x.y); }
+
+// Norm and rotation of one row piece; the row's lanes are consecutive and every
+// lane of the warp takes part.
+template <int DIM, bool PAIRED>
+__device__ __forceinline__ void turn_row(float2 (&x)[4], int l, const float* norm, const float2 (&w)[4], const Angles& g,
+                                         const b3_kv_append_args& a) {
+    if (norm) {
+        float2 ss2 = __fmul2_rn(x[0], x[0]);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) ss2 = __ffma2_rn(x[i], x[i], ss2);
+        float ss = ss2.x + ss2.y;
 #pragma unroll
         for (int m = DIM / 16; m; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-        const float r = 1.f / sqrtf(ss * (1.f / DIM) + a.eps);
-        const float4 w0 = __ldg(reinterpret_cast<const float4*>(norm) + 2 * l);
-        const float4 w1 = __ldg(reinterpret_cast<const float4*>(norm) + 2 * l + 1);
-        const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        const float r = rsqrtf(ss * (1.f / DIM) + a.eps);   // within 2 units in the last place
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+        for (int i = 0; i < 4; ++i) x[i] = __fmul2_rn(__fmul2_rn(x[i], make_float2(r, r)), w[i]);
     }
-    if (a.cos) {
-        const int half = a.rot_dim >> 1;
-        const int64_t row = static_cast<int64_t>(pos) * half;
-        const int ch = 8 * l;
+    if (PAIRED) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 u = x[i], v = x[2 + i];
+            x[i] = __ffma2_rn(u, g.c[i], neg2(__fmul2_rn(v, g.s[i])));
+            x[2 + i] = __ffma2_rn(v, g.c[i], __fmul2_rn(u, g.s[i]));
+        }
+    } else if (a.cos) {
+        const int half = a.rot_dim >> 1, ch = 8 * l;
         if (a.interleaved) {
             if (ch < a.rot_dim) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float c = __ldg(a.cos + row + (ch >> 1) + i), s = __ldg(a.sin + row + (ch >> 1) + i);
-                    const float u = x[2 * i], v = x[2 * i + 1];
-                    x[2 * i] = u * c - v * s;
-                    x[2 * i + 1] = v * c + u * s;
+                    const float c = i & 1 ? g.c[i >> 1].y : g.c[i >> 1].x, s = i & 1 ? g.s[i >> 1].y : g.s[i >> 1].x;
+                    x[i] = make_float2(x[i].x * c - x[i].y * s, x[i].y * c + x[i].x * s);
                 }
             }
         } else {
@@ -73,16 +175,15 @@ __device__ __forceinline__ void turn_row(float (&x)[8], int l, const float* norm
             const bool low = ch < half;
             const int lane = threadIdx.x & 31;
             const int from = low ? lane + (half >> 3) : lane - (half >> 3);
-            float y[8];
+            float2 y[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], from & 31);
+            for (int i = 0; i < 4; ++i) {
+                y[i].x = __shfl_sync(0xffffffffu, x[i].x, from & 31);
+                y[i].y = __shfl_sync(0xffffffffu, x[i].y, from & 31);
+            }
             if (ch < a.rot_dim) {
-                const int64_t at = row + (low ? ch : ch - half);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float c = __ldg(a.cos + at + i), s = __ldg(a.sin + at + i);
-                    x[i] = low ? x[i] * c - y[i] * s : x[i] * c + y[i] * s;
-                }
+                for (int i = 0; i < 4; ++i) x[i] = __ffma2_rn(x[i], g.c[i], __fmul2_rn(low ? neg2(y[i]) : y[i], g.s[i]));
             }
         }
     }
@@ -111,37 +212,39 @@ __device__ __forceinline__ bool seq_span(const AppendParams& p, int s, int& firs
     return fits;
 }
 
-template <typename T, int DIM, bool VEC>
+template <typename T, int DIM, bool VEC, bool PAIRED>
 __device__ __forceinline__ void q_rows(const AppendParams& p, int warp_id) {
+    using P = Piece<DIM, PAIRED>;
     constexpr int kLanes = DIM / 8, kRows = 32 / kLanes;
     const int token = warp_id / p.q_chunks;
     if (token >= p.b.tokens) return;
     const int lane = threadIdx.x & 31, l = lane % kLanes;
+    const int h0 = (warp_id % p.q_chunks) * kQRows * kRows + lane / kLanes;
+    const T* q = static_cast<const T*>(p.a.q) + token * p.a.q_token_stride + h0 * p.a.q_head_stride;
+    float2 x[kQRows][4];
+#pragma unroll
+    for (int r = 0; r < kQRows; ++r) {
+        if (h0 + r * kRows < p.a.q_heads)
+            P::template load<VEC>(q + r * kRows * p.a.q_head_stride, l, x[r]);
+        else
+            x[r][0] = x[r][1] = x[r][2] = x[r][3] = make_float2(0.f, 0.f);
+    }
     const int s = kv_seq_of(p.b, token);
     int first, begin, end;
     if (!seq_span(p, s, first, begin, end) || token - first < 0 || token - first >= end - begin) return;
-    const int pos = token_position(p, token, begin + token - first);
-    const int h0 = (warp_id % p.q_chunks) * kQRows * kRows + lane / kLanes;
-    float x[kQRows][8];
+    Angles g;
+    float2 w[4];
+    load_angles<DIM, PAIRED>(g, l, token_position(p, token, begin + token - first), p);
+    P::load_norm(w, p.a.q_norm, l);
+    const int64_t at = (static_cast<int64_t>(token) * p.a.q_heads + h0) * DIM;
 #pragma unroll
     for (int r = 0; r < kQRows; ++r) {
-        const int h = h0 + r * kRows;
-        if (h < p.a.q_heads)
-            load8<VEC>(static_cast<const T*>(p.a.q) + token * p.a.q_token_stride + h * p.a.q_head_stride + 8 * l, x[r]);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[r][i] = 0.f;
-    }
-#pragma unroll
-    for (int r = 0; r < kQRows; ++r) {
-        const int h = h0 + r * kRows;
-        turn_row<DIM>(x[r], l, p.a.q_norm, pos, p.a);
-        if (h < p.a.q_heads) {
-            const int64_t at = (static_cast<int64_t>(token) * p.a.q_heads + h) * DIM + 8 * l;
+        turn_row<DIM, PAIRED>(x[r], l, p.a.q_norm, w, g, p.a);
+        if (h0 + r * kRows < p.a.q_heads) {
             if (p.a.out_dtype == B3_DTYPE_F16)
-                store8(static_cast<__half*>(p.a.q_out) + at, x[r]);
+                P::store(static_cast<__half*>(p.a.q_out) + at + r * kRows * DIM, l, x[r]);
             else
-                store8(static_cast<__nv_bfloat16*>(p.a.q_out) + at, x[r]);
+                P::store(static_cast<__nv_bfloat16*>(p.a.q_out) + at + r * kRows * DIM, l, x[r]);
         }
     }
 }
@@ -149,8 +252,9 @@ __device__ __forceinline__ void q_rows(const AppendParams& p, int warp_id) {
 // One (page, key head, k or v).  GROUP warps of the block (all of it, or each
 // warp on its own), `gw` this warp's place in the group.  ROWS: passes of the
 // group over a full page; with ROWS > 0 the rows stay in registers.
-template <typename T, int DIM, bool VEC, int GROUP, int ROWS>
+template <typename T, int DIM, bool VEC, bool PAIRED, int GROUP, int ROWS>
 __device__ __forceinline__ void cache_unit(const AppendParams& p, int item, int gw, float* xmax) {
+    using P = Piece<DIM, PAIRED>;
     constexpr int kLanes = DIM / 8, kRows = 32 / kLanes, kStep = kRows * GROUP;
     const int heads = p.c.kv_heads, page = p.c.page_tokens;
     const int unit = item / (2 * heads), which = (item / heads) & 1, head = item % heads;
@@ -183,27 +287,30 @@ __device__ __forceinline__ void cache_unit(const AppendParams& p, int item, int 
     uint8_t* const codes = (which ? p.c.v : p.c.k) + slab * page * DIM;
     const float old_scale = held ? *scale_at : 0.f;
 
-    auto load_row = [&](int r, float (&x)[8]) {   // new row r of the page, zero past the last; whole warps
-        const int token = first + lo - begin + r;
-        if (r < rows) {
-            if (which)
-                load8<VEC>(static_cast<const T*>(p.a.v) + token * p.a.v_token_stride + head * p.a.v_head_stride + 8 * l, x);
-            else
-                load8<VEC>(static_cast<const T*>(p.a.k) + token * p.a.k_token_stride + head * p.a.k_head_stride + 8 * l, x);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        }
+    const int token0 = first + lo - begin;
+    const T* const from = which ? static_cast<const T*>(p.a.v) + token0 * p.a.v_token_stride + head * p.a.v_head_stride
+                                : static_cast<const T*>(p.a.k) + token0 * p.a.k_token_stride + head * p.a.k_head_stride;
+    const int64_t stride = which ? p.a.v_token_stride : p.a.k_token_stride;
+    auto load_row = [&](int r, float2 (&x)[4]) {   // new row r of the page, zero past the last; whole warps
+        if (r < rows)
+            P::template load<VEC>(from + r * stride, l, x);
+        else
+            x[0] = x[1] = x[2] = x[3] = make_float2(0.f, 0.f);
     };
-    auto turn = [&](int r, float (&x)[8]) {
-        if (!which) turn_row<DIM>(x, l, p.a.k_norm, r < rows ? token_position(p, first + lo - begin + r, lo + r) : 0, p.a);
+    float2 w[4];
+    if (!which) P::load_norm(w, p.a.k_norm, l);
+    auto turn = [&](int r, float2 (&x)[4]) {
+        if (which) return;
+        Angles g;
+        load_angles<DIM, PAIRED>(g, l, r < rows ? token_position(p, token0 + r, lo + r) : 0, p);
+        turn_row<DIM, PAIRED>(x, l, p.a.k_norm, w, g, p.a);
     };
-    auto code_row = [&](int r, const float (&x)[8], float inv) {
-        if (r < rows) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(held + r) * DIM + 8 * l) = encode8(x, inv);
+    auto code_row = [&](int r, const float2 (&x)[4], float inv) {
+        if (r < rows) P::store_codes(codes + static_cast<int64_t>(held + r) * DIM, l, x, inv);
     };
 
     constexpr int kKeep = ROWS > 0 ? ROWS : 1;
-    float x[kKeep][8];
+    float2 x[kKeep][4];
     float amax = 0.f;
     if (ROWS > 0) {
 #pragma unroll
@@ -212,14 +319,14 @@ __device__ __forceinline__ void cache_unit(const AppendParams& p, int item, int 
         for (int k = 0; k < kKeep; ++k) {
             turn(row + k * kStep, x[k]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(x[k][i]));
+            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(finite_abs(x[k][i].x), finite_abs(x[k][i].y)));
         }
     } else {
         for (int r = row; r - lane / kLanes < rows; r += kStep) {
             load_row(r, x[0]);
             turn(r, x[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, finite_abs(x[0][i]));
+            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(finite_abs(x[0][i].x), finite_abs(x[0][i].y)));
         }
     }
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
@@ -261,28 +368,28 @@ __device__ __forceinline__ void cache_unit(const AppendParams& p, int item, int 
     if (gw == 0 && lane == 0) *scale_at = exp2_int(e);
 }
 
-template <typename T, int DIM, bool VEC, int GROUP, int ROWS>
-__global__ void __launch_bounds__(kThreads) k_kv_append(const __grid_constant__ AppendParams p) {
+template <typename T, int DIM, bool VEC, bool PAIRED, int GROUP, int ROWS>
+__global__ void __launch_bounds__(kThreads, ROWS >= 8 ? 2 : 3) k_kv_append(const __grid_constant__ AppendParams p) {
     __shared__ float xmax[kWarps];
     const int warp = threadIdx.x >> 5;
     if (static_cast<int>(blockIdx.x) < p.kv_blocks) {
         if (GROUP > 1)
-            cache_unit<T, DIM, VEC, GROUP, ROWS>(p, blockIdx.x, warp, xmax);
+            cache_unit<T, DIM, VEC, PAIRED, GROUP, ROWS>(p, blockIdx.x, warp, xmax);
         else
-            cache_unit<T, DIM, VEC, GROUP, ROWS>(p, blockIdx.x * kWarps + warp, 0, xmax);
+            cache_unit<T, DIM, VEC, PAIRED, GROUP, ROWS>(p, blockIdx.x * kWarps + warp, 0, xmax);
     } else {
-        q_rows<T, DIM, VEC>(p, (blockIdx.x - p.kv_blocks) * kWarps + warp);
+        q_rows<T, DIM, VEC, PAIRED>(p, (blockIdx.x - p.kv_blocks) * kWarps + warp);
     }
 }
 
-template <typename T, int DIM, bool VEC, int GROUP, int ROWS>
+template <typename T, int DIM, bool VEC, bool PAIRED, int GROUP, int ROWS>
 int launch(const AppendParams& p, int64_t blocks, cudaStream_t st) {
-    k_kv_append<T, DIM, VEC, GROUP, ROWS><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(p);
+    k_kv_append<T, DIM, VEC, PAIRED, GROUP, ROWS><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(p);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : set_cuda_error("k_kv_append", e);
 }
 
-template <typename T, int DIM, bool VEC>
+template <typename T, int DIM, bool VEC, bool PAIRED>
 int launch_dim(AppendParams& p, cudaStream_t st) {
     constexpr int kRows = 32 / (DIM / 8);
     const int page = p.c.page_tokens;
@@ -302,12 +409,12 @@ int launch_dim(AppendParams& p, cudaStream_t st) {
         return set_error(B3_EINVAL, "b3_kv_append: %lld tokens are too many for one call",
                          static_cast<long long>(p.b.tokens));
     p.kv_blocks = static_cast<int>(kv_blocks);
-    if (!whole) return launch<T, DIM, VEC, 1, 0>(p, blocks, st);
+    if (!whole) return launch<T, DIM, VEC, PAIRED, 1, 0>(p, blocks, st);
     switch (page / (kRows * kWarps)) {
-        case 8: return launch<T, DIM, VEC, kWarps, 8>(p, blocks, st);
-        case 4: return launch<T, DIM, VEC, kWarps, 4>(p, blocks, st);
-        case 2: return launch<T, DIM, VEC, kWarps, 2>(p, blocks, st);
-        default: return launch<T, DIM, VEC, kWarps, 1>(p, blocks, st);
+        case 8: return launch<T, DIM, VEC, PAIRED, kWarps, 8>(p, blocks, st);
+        case 4: return launch<T, DIM, VEC, PAIRED, kWarps, 4>(p, blocks, st);
+        case 2: return launch<T, DIM, VEC, PAIRED, kWarps, 2>(p, blocks, st);
+        default: return launch<T, DIM, VEC, PAIRED, kWarps, 1>(p, blocks, st);
     }
 }
 
@@ -319,8 +426,13 @@ int launch_type(AppendParams& p, cudaStream_t st) {
     const int64_t strides = a.q_token_stride | a.q_head_stride | a.k_token_stride | a.k_head_stride |
                             a.v_token_stride | a.v_head_stride;
     const bool vec = bases % 16 == 0 && strides % per16 == 0;
-    if (p.c.head_dim == 128) return vec ? launch_dim<T, 128, true>(p, st) : launch_dim<T, 128, false>(p, st);
-    return vec ? launch_dim<T, 64, true>(p, st) : launch_dim<T, 64, false>(p, st);
+    const bool paired = a.cos && !a.interleaved && a.rot_dim == p.c.head_dim;
+    if (p.c.head_dim == 128) {
+        if (paired) return vec ? launch_dim<T, 128, true, true>(p, st) : launch_dim<T, 128, false, true>(p, st);
+        return vec ? launch_dim<T, 128, true, false>(p, st) : launch_dim<T, 128, false, false>(p, st);
+    }
+    if (paired) return vec ? launch_dim<T, 64, true, true>(p, st) : launch_dim<T, 64, false, true>(p, st);
+    return vec ? launch_dim<T, 64, true, false>(p, st) : launch_dim<T, 64, false, false>(p, st);
 }
 
 }  // namespace
@@ -373,6 +485,7 @@ extern "C" int b3_kv_append(const b3_kv_cache* cache, const b3_kv_batch* batch, 
     p.c = *cache;
     p.b = *batch;
     p.a = a;
+    p.angles16 = ((reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) & 15) == 0;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (a.dtype) {
         case B3_DTYPE_F32: return launch_type<float>(p, st);
