@@ -16,10 +16,11 @@
 // the row.  PAIRED (the usual rotation of all channels, i with i + head_dim / 2)
 // gives a lane four channels and their four partners, so the rotation stays in
 // the lane; otherwise a lane has eight neighbours and shuffles for partners.
-//   GROUP = 1: a warp a (page, head).  Decode brings one row to each page.
-//   GROUP = 8: a whole block, the page's rows in registers between the
-//              exponent and the codes.  Prompts fill whole pages.
-// The host takes GROUP = 8 from four new tokens a sequence on average.
+//   GROUP = 1     a warp a (page, head).  Decode brings one row to each page.
+//   GROUP = 4, 8  that many warps, the page's rows in registers between the
+//                 exponent and the codes.  Prompts fill whole pages; four warps
+//                 hold 16 rows of 64 channels.
+// The host takes groups from four new tokens a sequence on average.
 #include "kv_cache.cuh"
 
 namespace b3 {
@@ -319,7 +320,14 @@ __device__ __forceinline__ void cache_unit(const AppendParams& p, int item, int 
         for (int k = 0; k < kKeep; ++k) {
             turn(row + k * kStep, x[k]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(finite_abs(x[k][i].x), finite_abs(x[k][i].y)));
+            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y)));
+        }
+        if (__any_sync(0xffffffffu, amax == INFINITY)) {   // infinities have no say in a scale (nor NaN, which fmaxf passes over)
+            amax = 0.f;
+#pragma unroll
+            for (int k = 0; k < kKeep; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fmaxf(finite_abs(x[k][i].x), finite_abs(x[k][i].y)));
         }
     } else {
         for (int r = row; r - lane / kLanes < rows; r += kStep) {
@@ -330,9 +338,9 @@ __device__ __forceinline__ void cache_unit(const AppendParams& p, int item, int 
         }
     }
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-    if (GROUP > 1) {   // every thread of the block is here: the early exits above are the same for all of it
+    if (GROUP > 1) {   // the group's warps are all here: the early exits above are the same for all of them
         if (lane == 0) xmax[gw] = amax;
-        __syncthreads();
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / (32 * GROUP)), "n"(32 * GROUP) : "memory");
 #pragma unroll
         for (int w = 0; w < GROUP; ++w) amax = fmaxf(amax, xmax[w]);
     }
@@ -373,10 +381,8 @@ __global__ void __launch_bounds__(kThreads, ROWS >= 8 ? 2 : 3) k_kv_append(const
     __shared__ float xmax[kWarps];
     const int warp = threadIdx.x >> 5;
     if (static_cast<int>(blockIdx.x) < p.kv_blocks) {
-        if (GROUP > 1)
-            cache_unit<T, DIM, VEC, PAIRED, GROUP, ROWS>(p, blockIdx.x, warp, xmax);
-        else
-            cache_unit<T, DIM, VEC, PAIRED, GROUP, ROWS>(p, blockIdx.x * kWarps + warp, 0, xmax);
+        const int group = warp / GROUP;
+        cache_unit<T, DIM, VEC, PAIRED, GROUP, ROWS>(p, blockIdx.x * (kWarps / GROUP) + group, warp % GROUP, xmax + group * GROUP);
     } else {
         q_rows<T, DIM, VEC, PAIRED>(p, (blockIdx.x - p.kv_blocks) * kWarps + warp);
     }
@@ -403,18 +409,21 @@ int launch_dim(AppendParams& p, cudaStream_t st) {
     const int64_t items = static_cast<int64_t>(p.units) * 2 * p.c.kv_heads;
     const int64_t q_warps = static_cast<int64_t>(p.b.tokens) * p.q_chunks;
     const bool whole = p.b.tokens >= 4ll * p.b.n_seq;
-    const int64_t kv_blocks = whole ? items : (items + kWarps - 1) / kWarps;
+    const int passes = page / (kRows * kWarps);
+    const int group = !whole ? 1 : passes ? kWarps : 4;
+    const int64_t kv_blocks = (items * group + kWarps - 1) / kWarps;
     const int64_t blocks = kv_blocks + (q_warps + kWarps - 1) / kWarps;
     if (blocks > 0x7fffffffll || items > 0x7fffffffll || q_warps > 0x7fffffffll)
         return set_error(B3_EINVAL, "b3_kv_append: %lld tokens are too many for one call",
                          static_cast<long long>(p.b.tokens));
     p.kv_blocks = static_cast<int>(kv_blocks);
     if (!whole) return launch<T, DIM, VEC, PAIRED, 1, 0>(p, blocks, st);
-    switch (page / (kRows * kWarps)) {
+    switch (passes) {
         case 8: return launch<T, DIM, VEC, PAIRED, kWarps, 8>(p, blocks, st);
         case 4: return launch<T, DIM, VEC, PAIRED, kWarps, 4>(p, blocks, st);
         case 2: return launch<T, DIM, VEC, PAIRED, kWarps, 2>(p, blocks, st);
-        default: return launch<T, DIM, VEC, PAIRED, kWarps, 1>(p, blocks, st);
+        case 1: return launch<T, DIM, VEC, PAIRED, kWarps, 1>(p, blocks, st);
+        default: return launch<T, DIM, VEC, PAIRED, 4, 1>(p, blocks, st);
     }
 }
 
