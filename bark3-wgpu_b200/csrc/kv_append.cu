@@ -377,7 +377,7 @@ __device__ __forceinline__ void cache_unit(const AppendParams& p, int item, int 
 }
 
 template <typename T, int DIM, bool VEC, bool PAIRED, int GROUP, int ROWS>
-__global__ void __launch_bounds__(kThreads, ROWS >= 8 ? 2 : 3) k_kv_append(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kThreads, ROWS >= 8 ? 2 : 4) k_kv_append(const __grid_constant__ AppendParams p) {
     __shared__ float xmax[kWarps];
     const int warp = threadIdx.x >> 5;
     if (static_cast<int>(blockIdx.x) < p.kv_blocks) {
