@@ -6,8 +6,10 @@
 // tile).  The mathematics is in kv_attend.cuh.
 //
 // Work.  The steps of 32 keys of all (sequence, key head) items, laid end to
-// end, are cut into equal runs, one for each resident warp, so ragged batches
-// and one long sequence keep every SM reading to the end.  A warp carries the
+// end with four more units for the start of each item (without them the warps
+// that get the shortest sequences, a dozen of them, finish last: 94 against 63
+// us for a ragged batch of 128), are cut into equal runs, one for each resident
+// warp, so ragged batches and one long sequence keep every SM reading to the end.  A warp carries the
 // running maximum, sum and output of its item in registers; a run that covers
 // an item from end to end stores the result, other runs leave partial results
 // that k_join adds up in run order (same bits every time).
@@ -40,7 +42,7 @@ namespace {
 constexpr int kStep = 32;           // keys
 constexpr int kTilesM = kStep / 16; // MMA tiles of 16 keys
 constexpr int kMaxSeqs = 1024;      // sequences a launch
-constexpr int kMinRun = 2;          // steps a run at least
+constexpr int kItem = 4;            // what starting an item costs, in steps
 
 template <int DIM, int ROWS>
 struct Cfg {
@@ -108,23 +110,23 @@ __device__ __forceinline__ void item_keys(const AttendParams& p, const SeqSpan& 
     lo = min(lo, hi) / kStep * kStep;
 }
 
-// Steps of one key head of a sequence: at least one where it has queries, so
-// that rows that see nothing are written too.
-__device__ __forceinline__ int seq_steps(const RowsParams& r, int s) {
+// Units of one key head of a sequence: kItem and its steps, of which there is
+// at least one where it has queries, so that rows that see nothing are written.
+__device__ __forceinline__ int seq_units(const RowsParams& r, int s) {
     SeqSpan sp = attend_span(r.p, r.seq0 + s);
     if (sp.n == 0) return 0;
     int lo, hi;
     item_keys(r.p, sp, lo, hi);
-    return max(1, (hi - lo + kStep - 1) / kStep);
+    return kItem + max(1, (hi - lo + kStep - 1) / kStep);
 }
 
-// prefix[i] = steps of one key head in the sequences before i, by the whole block.
+// prefix[i] = units of one key head in the sequences before i, by the whole block.
 __device__ __forceinline__ void make_prefix(const RowsParams& r, int* prefix, int* warp_sums) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nwarps = blockDim.x >> 5;
     int carry = 0;
     for (int base = 0; base < r.seqs; base += blockDim.x) {
         const int s = base + tid;
-        int v = s < r.seqs ? seq_steps(r, s) : 0;
+        int v = s < r.seqs ? seq_units(r, s) : 0;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, v, d);
@@ -146,11 +148,11 @@ __device__ __forceinline__ void make_prefix(const RowsParams& r, int* prefix, in
     __syncthreads();
 }
 
-// Item and first step of global step g: heads of a sequence follow one another.
+// The item of global unit g: heads of a sequence follow one another.
 struct Place {
     int seq, head;       // seq within the launch
-    int64_t begin;       // global step of the item's first
-    int steps;
+    int64_t begin;       // global unit of the item's first
+    int units;
 };
 __device__ __forceinline__ Place place_of(const int* prefix, int n, int heads, int64_t g) {
     int lo = 0, hi = n;   // prefix[lo] * heads <= g < prefix[hi] * heads
@@ -160,15 +162,15 @@ __device__ __forceinline__ Place place_of(const int* prefix, int n, int heads, i
     }
     Place q;
     q.seq = lo;
-    q.steps = prefix[lo + 1] - prefix[lo];
+    q.units = prefix[lo + 1] - prefix[lo];
     const int64_t base = static_cast<int64_t>(prefix[lo]) * heads;
-    q.head = static_cast<int>((g - base) / q.steps);
-    q.begin = base + static_cast<int64_t>(q.head) * q.steps;
+    q.head = static_cast<int>((g - base) / q.units);
+    q.begin = base + static_cast<int64_t>(q.head) * q.units;
     return q;
 }
 
 __device__ __forceinline__ int64_t run_length(int64_t total, int workers) {
-    return max(static_cast<int64_t>(kMinRun), (total + workers - 1) / workers);
+    return max(static_cast<int64_t>(1), (total + workers - 1) / workers);
 }
 
 template <typename T, int N>
@@ -217,12 +219,14 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
 
     while (at < end) {
         const Place it = place_of(prefix, r.seqs, heads, at);
+        const int64_t upto = min(end, it.begin + it.units), from = at;
+        at = upto;
+        const int s0 = max(0, static_cast<int>(from - it.begin) - kItem), s1 = static_cast<int>(upto - it.begin) - kItem;
+        if (s1 <= s0) continue;   // only the item's start
         const int seq = r.seq0 + it.seq;
         const SeqSpan sp = attend_span(p, seq);
         int key_lo, key_hi;
         item_keys(p, sp, key_lo, key_hi);
-        const int s0 = static_cast<int>(at - it.begin);
-        const int s1 = static_cast<int>(min(end - it.begin, static_cast<int64_t>(it.steps)));
         const int key0 = key_lo + s0 * kStep;                 // this run's keys of the item: [key0, key1)
         const int key1 = min(key_lo + s1 * kStep, key_hi);
         const int n_steps = key1 > key0 ? (key1 - key0 + kStep - 1) / kStep : 0;
@@ -380,11 +384,14 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
                 const int i = (key >> log_page) - page0;
                 ks[0] = __shfl_sync(0xffffffffu, ks_a, i);
                 ve[0] = stored_exp(__shfl_sync(0xffffffffu, vs_a, i));
-                ks[1] = ks[0];
-                ve[1] = ve[0];
-                if (page < kStep) {
-                    ks[1] = __shfl_sync(0xffffffffu, ks_a, i + 1);
-                    ve[1] = stored_exp(__shfl_sync(0xffffffffu, vs_a, i + 1));
+#pragma unroll
+                for (int mt = 1; mt < kTilesM; ++mt) {
+                    ks[mt] = ks[0];
+                    ve[mt] = ve[0];
+                    if (page < kStep) {
+                        ks[mt] = __shfl_sync(0xffffffffu, ks_a, i + mt);
+                        ve[mt] = stored_exp(__shfl_sync(0xffffffffu, vs_a, i + mt));
+                    }
                 }
             }
             const uint32_t st = used % C::kStages;
@@ -529,8 +536,8 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
         }
 
         // ── the run's end: rows' sums over the eight lanes that share them ──
-        const bool all = s0 == 0 && s1 == it.steps;
-        const int64_t slot = 2ll * worker + (at > worker * run ? 1 : 0);
+        const bool all = s0 == 0 && s1 == it.units - kItem;
+        const int64_t slot = 2ll * worker + (from > worker * run ? 1 : 0);
 #pragma unroll
         for (int hf = 0; hf < kHalves; ++hf)
 #pragma unroll
@@ -560,7 +567,6 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
                 }
             }
         if (!ok) break;
-        at = it.begin + s1;
     }
 }
 
@@ -577,14 +583,15 @@ __global__ void __launch_bounds__(kJoinMax * 32) k_attend_join(const __grid_cons
     make_prefix(r, prefix, prefix + kMaxSeqs + 1);
     const AttendParams& p = r.p;
     const int heads = p.c.kv_heads, group = p.a.q_heads / heads;
-    const int seq = blockIdx.x / heads, head = blockIdx.x % heads, steps = prefix[seq + 1] - prefix[seq];
+    const int seq = blockIdx.x / heads, head = blockIdx.x % heads, units = prefix[seq + 1] - prefix[seq];
     const int64_t run = run_length(static_cast<int64_t>(prefix[r.seqs]) * heads, r.workers);
-    const int64_t begin = static_cast<int64_t>(prefix[seq]) * heads + static_cast<int64_t>(head) * steps;
-    const int w0 = static_cast<int>(begin / run), w1 = static_cast<int>((begin + steps - 1) / run);
+    const int64_t begin = static_cast<int64_t>(prefix[seq]) * heads + static_cast<int64_t>(head) * units;
+    // the runs that hold its first and its last step
+    const int w0 = static_cast<int>((begin + kItem) / run), w1 = static_cast<int>((begin + units - 1) / run);
     const int slot0 = begin > w0 * run ? 1 : 0;
     const SeqSpan sp = attend_span(p, r.seq0 + seq);
     pdl_wait();   // the partial results are complete (and this kernel ends after the one before it)
-    if (steps == 0 || w0 == w1) return;
+    if (units == 0 || w0 == w1) return;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int rows = sp.n * group;
