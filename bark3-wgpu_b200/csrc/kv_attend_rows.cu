@@ -552,10 +552,10 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
                 for (int j = 0; j < kSteps; ++j) x[2 * j] = o[hf][j][e], x[2 * j + 1] = o[hf][j][2 + e];
                 if (all) {
                     const int token = sp.first + row / group, head = it.head * group + row % group;
-                    store_row<T>(p, token, head, 2 * kSteps * g, x, sum == 0.f ? 0.f : 1.f / sum);
+                    store_row<T>(p, token, head, 2 * kSteps * g, x, row_inverse(sum));
                     if (p.a.lse && g == 0)
                         p.a.lse[static_cast<int64_t>(token) * p.a.q_heads + head] =
-                            sum == 0.f ? -INFINITY : (m[hf][e] + log2f(sum)) * kLn2;
+                            row_lse(m[hf][e], sum);
                 } else {
                     float* po = r.part + (slot * ROWS + row) * DIM + 2 * kSteps * g;
 #pragma unroll
@@ -567,6 +567,41 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
                 }
             }
         if (!ok) break;
+        if (sp.n > 1 && p.a.causal) {
+            // rows that came out NaN (or infinite), where rows see different keys: again, without the keys they do not see
+            __syncwarp();
+#pragma unroll
+            for (int hf = 0; hf < kHalves; ++hf)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float nan = 0.f;
+#pragma unroll
+                    for (int j = 0; j < kSteps; ++j) nan = fmaf(o[hf][j][e], 0.f, fmaf(o[hf][j][2 + e], 0.f, nan));
+                    const unsigned bad = __ballot_sync(0xffffffffu, nan != nan);   // lane 4 g + t: a part of row 2 t + e
+                    for (int c = 0; c < 4; ++c) {
+                        const int row = 2 * c + e + 8 * hf;
+                        if (!(bad & (0x11111111u << c)) || row >= n_rows) continue;
+                        const int i = row / group, head = it.head * group + row % group;
+                        float x[DIM / 32], mm, ll;
+                        attend_row_exact<T, DIM>(p, seq, sp.first + i, i, head, key0, key1, x, mm, ll);
+                        const int64_t out = static_cast<int64_t>(sp.first + i) * p.a.q_heads + head;
+                        for (int d = 0; d < DIM / 32; ++d) {
+                            const int ch = lane * (DIM / 32) + d;
+                            if (all)
+                                from_f32(x[d] * row_inverse(ll), static_cast<T*>(p.a.out)[out * DIM + ch]);
+                            else
+                                r.part[(slot * ROWS + row) * DIM + ch] = x[d];
+                        }
+                        if (lane == 0) {
+                            if (!all)
+                                *reinterpret_cast<float2*>(r.part + 2ll * r.workers * ROWS * DIM + (slot * ROWS + row) * 2) =
+                                    make_float2(mm, ll);
+                            else if (p.a.lse)
+                                p.a.lse[out] = row_lse(mm, ll);
+                        }
+                    }
+                }
+        }
     }
 }
 
@@ -644,10 +679,10 @@ __global__ void __launch_bounds__(kJoinMax * 32) k_attend_join(const __grid_cons
         if (live && mine == 0) {
             const int token = sp.first + row / group, q_head = head * group + row % group;
             const int64_t at = static_cast<int64_t>(token) * p.a.q_heads + q_head;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = row_inverse(l);
 #pragma unroll
             for (int i = 0; i < kPer; ++i) from_f32(o[i] * inv, static_cast<T*>(p.a.out)[at * DIM + lane * kPer + i]);
-            if (p.a.lse && lane == 0) p.a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+            if (p.a.lse && lane == 0) p.a.lse[at] = row_lse(m, l);
         }
     }
 }

@@ -433,6 +433,38 @@ def test_attend_nan_reaches_only_who_sees_it(pkg, max_q):
     assert bad[cu[1]:cu[2], :2].all() and bad.sum() == n * 2 * dim
 
 
+@pytest.mark.parametrize("n,q_heads,window", [(4, 4, 0), (3, 10, 8), (100, 4, 0), (300, 6, 20)])
+def test_attend_masked_nan_stays_masked(pkg, n, q_heads, window):
+    """A NaN value (and a NaN key) of a new token: the tokens before it, and those whose window is past it, do not see it."""
+    rng = np.random.default_rng(n)
+    page, dim, kv_heads = 16, 64, 2
+    dev, cu, kv, table, pages = make_batch(rng, page, [50, 3], [n, n])
+    q = torch.from_numpy(rng.normal(0, 1, (int(cu[-1]), q_heads, dim)).astype(np.float32)).half().cuda()
+    clean = random_cache(pkg, rng, pages, kv_heads, page, dim)
+    at = kv[0] - n + n // 2                     # the middle one of the new tokens of sequence 0
+    want, want_lse = clean.attend(q, **dev, max_q=n, scale=0.02, window=window, return_lse=True)
+    for pool in (clean.v, clean.k):
+        cell = pool.view(torch.uint8)[table[0, at // page], 1, at % page]
+        keep = cell.clone()
+        cell[5] = 0x7F
+        out, lse = clean.attend(q, **dev, max_q=n, scale=0.02, window=window, return_lse=True)
+        cell.copy_(keep)
+        clean.check()
+        sees = np.zeros(int(cu[-1]), bool)
+        sees[n // 2:n if not window else min(n, n // 2 + window)] = True
+        group = q_heads // kv_heads
+        bad = torch.isnan(out).cpu().numpy()
+        if pool is clean.v:
+            assert bad[sees][:, group:, 5].all() and bad.sum() == sees.sum() * group
+        else:
+            assert bad[sees][:, group:].all() and bad.sum() == sees.sum() * group * dim
+        # who does not see it: as before, but for the order in which rows taken again add up (f32, probabilities not rounded)
+        d = (out.float() - want.float()).abs().cpu().numpy()
+        assert (d[~bad] <= 2.0 ** -9 * np.abs(want.float().cpu().numpy()).max()).all()
+        fine = ~np.isnan(lse.cpu().numpy())
+        assert np.allclose(lse.cpu().numpy()[fine], want_lse.cpu().numpy()[fine], rtol=1e-5, atol=1e-5)
+
+
 def test_attend_strides_streams_and_repeats(pkg):
     """Query views, a side stream, and the same bits every time."""
     rng = np.random.default_rng(4)
