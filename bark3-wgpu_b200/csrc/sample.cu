@@ -9,7 +9,7 @@
 // total.
 //
 // A row is read once, into the shared memory of a cluster of 1 to 8 blocks of
-// 512 threads (a column of values for each thread, in their own type, touched
+// 512 threads (a column of vectors for each thread, in their own type, touched
 // by it alone; a warp's values are neighbours in the row, in index order over
 // (vector, lane, place)).  Shared memory and not registers: loops over 32
 // values unrolled with an exponential in each miss the instruction cache.
@@ -30,6 +30,8 @@
 //   long ties      A list that overflows (thousands of equal logits) falls back
 //                  to a search over the bits of (logit, index).
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "kv_cache.cuh"
 
@@ -84,21 +86,28 @@ __device__ __forceinline__ u64 rank_key(float x, int i) { return static_cast<u64
 // on the IBM RISC System/6000 processor", 1990); such t, and ones so far out
 // that a residual could leave the normal range, are divided by.
 struct Weigh {
-    float peak, t, inv;
-    bool divide;
+    float peak, t, inv, least;
+    bool divide, infinite;
     __device__ __forceinline__ void set(float p, float temperature) {
         peak = p;
         t = temperature;
         inv = __frcp_rn(t);
+        least = -64.f * t;   // exp(-64) is no weight: what is further down is held here
         divide = (__float_as_uint(t) & 0x7fffffu) == 0x7fffffu || !(t > 0x1p-60f && t < 0x1p60f);
+        infinite = peak == INFINITY;
     }
-    __device__ __forceinline__ float power(float x) const {
-        const float a = x - peak;
-        if (divide || !(a > -0x1p60f)) return a / t;
-        const float q = a * inv;
+    // the usual row: no branch and no division, in loops over all values
+    __device__ __forceinline__ bool usual() const { return !divide && !infinite; }
+    __device__ __forceinline__ float usual_power(float x) const {
+        const float a = fmaxf(x - peak, least), q = a * inv;
         return fmaf(fmaf(-q, t, a), inv, q);
     }
-    __device__ __forceinline__ float operator()(float x) const { return x == peak ? 1.f : expf(power(x)); }
+    __device__ __forceinline__ float power(float x) const {
+        if (infinite) return x == peak ? 0.f : -INFINITY;
+        return divide ? (x - peak) / t : usual_power(x);
+    }
+    template <bool USUAL>
+    __device__ __forceinline__ float weight(float x) const { return expf(USUAL ? usual_power(x) : power(x)); }
 };
 __device__ __forceinline__ u32 whole(float w) { return static_cast<u32>(w * 2147483648.f); }
 
@@ -141,7 +150,7 @@ struct Row {
     __device__ __forceinline__ float at(int i) const { return to_f32(x[i]); }
 
     // The thread's values into its column, their maximum; what is no number, or outside the row, is -inf.
-    __device__ __forceinline__ float load(T* col) const {
+    __device__ __forceinline__ float load(uint4* col) const {
         T least;
         from_f32(-INFINITY, least);
         float top = -INFINITY;
@@ -158,18 +167,15 @@ struct Row {
                 const int e = c0 + c * kVec, i = index(e);
                 if (e >= count) break;
                 const bool vector = i >= 0 && i + kVec <= n && !by_one;
-                const T* t = reinterpret_cast<const T*>(&raw[c]);
+                T* t = reinterpret_cast<T*>(&raw[c]);
 #pragma unroll
                 for (int k = 0; k < kVec; ++k) {
-                    T y = least;
-                    if (vector)
-                        y = t[k];
-                    else if (i + k >= 0 && i + k < n)
-                        y = x[i + k];
-                    const float f = to_f32(y);
+                    if (!vector) t[k] = i + k >= 0 && i + k < n ? x[i + k] : least;
+                    const float f = to_f32(t[k]);
                     top = fmaxf(top, f);
-                    col[(e + k) * kThreads] = f > -INFINITY ? y : least;
+                    if (f != f) t[k] = least;
                 }
+                col[e / kVec * kThreads] = raw[c];
             }
         }
         return top;
@@ -212,8 +218,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     const int blocks = cluster.num_blocks(), me = cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / blocks;
     Shared* const first = cluster.map_shared_rank(&s, 0);
-    T* const col = reinterpret_cast<T*>(values) + tid;
-    auto value = [&](int e) { return to_f32(col[e * kThreads]); };
+    constexpr int kVec = Row<T>::kVec;
+    uint4* const col = values + tid;      // vector c of the thread at col[c * kThreads]
+    auto each = [&](auto f) {             // f(value, e) for the thread's values, rising indices
+#pragma unroll 2
+        for (int c = 0; c < count / kVec; ++c) {
+            const uint4 raw = col[c * kThreads];
+            const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) f(to_f32(t[k]), c * kVec + k);
+        }
+    };
 
     Row<T> r;
     r.x = static_cast<const T*>(a.logits) + row * a.row_stride;
@@ -288,8 +303,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     }
     if (!sampled) {
         int best = r.n;
-        for (int e = count - 1; e >= 0; --e)
-            if (value(e) == peak) best = r.index(e);
+        each([&](float x, int e) {
+            if (x == peak) best = min(best, r.index(e));
+        });
         best = __reduce_min_sync(0xffffffffu, best);
         if (lane == 0 && best < r.n) atomicMin(&first->best, best);
         cluster.sync();
@@ -307,11 +323,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
 
     // ── small top_k: candidates only ──
     if (by_list) {
-#pragma unroll 8
-        for (int e = 0; e < count; ++e) {
-            const float x = value(e);
+        each([&](float x, int e) {
             if (x >= jth && x > -INFINITY) enlist(x, r.index(e));
-        }
+        });
         cluster.sync();
         const int n = first->count;
         if (n <= kList) {
@@ -333,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
             float w = 0.f;
             if (tid < k) {
                 mine = s.list.key[tid];
-                w = weigh(logit_of(static_cast<u32>(mine >> 32)));
+                w = weigh.weight<false>(logit_of(static_cast<u32>(mine >> 32)));
             }
             u32 W = tid < k ? whole(w) : 0;
             if (top_p < 1.f) {
@@ -366,11 +380,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
         if (me == 0 && tid == 0) s.count = 0;
     }
 
+    auto rest = [&](auto usual) {
+    constexpr bool kUsual = decltype(usual)::value;
     // ── top_k (by counts), then top_p (by weights): a beginning of the order ──
     float cut_x = -INFINITY;   // kept: logits above it, and equal ones up to index cut_i
     int cut_i = -1;
     auto kept = [&](float x, int e) { return x > cut_x || (x == cut_x && r.index(e) <= cut_i); };
-    auto weight = [&](float x) { return whole(weigh(x)); };
+    auto weight = [&](float x) { return whole(weigh.template weight<kUsual>(x)); };
     // steps below the largest logit, the last one all of what weighs nothing: exp(-21.6) < 2^-31
     const float step = static_cast<float>(kBins - 1) / (21.6f * t);
     auto bin_of = [&](float x) {
@@ -383,10 +399,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
         for (int i = tid; i < kBins; i += kThreads) s.hist.lo[i] = s.hist.hi[i] = 0;
         if (tid == 0) s.cut_bin = -1;
         __syncthreads();
-#pragma unroll 4
-        for (int e = 0; e < count; ++e) {
-            const float x = value(e);
-            if (!kept(x, e)) continue;
+        each([&](float x, int e) {
+            if (!kept(x, e)) return;
             const int b = bin_of(x);
             if (stage == 0) {
                 atomicAdd(&s.hist.lo[b], 1u);
@@ -395,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
                 atomicAdd(&s.hist.lo[b], w & 0xffffu);
                 if (w >> 16) atomicAdd(&s.hist.hi[b], w >> 16);
             }
-        }
+        });
         cluster.sync();
         // each block adds up its share of the bins, the largest logits first, over all blocks
         const int share = kBins / blocks, per = (share + kThreads - 1) / kThreads;
@@ -435,11 +449,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
         if (cut < 0 || cut == kBins - 1) continue;   // only what weighs nothing would go
         const u64 above = s.cut_before;
         auto member = [&](float x, int e) { return kept(x, e) && bin_of(x) == cut; };
-#pragma unroll 4
-        for (int e = 0; e < count; ++e) {
-            const float x = value(e);
+        each([&](float x, int e) {
             if (member(x, e)) enlist(x, r.index(e));
-        }
+        });
         cluster.sync();
         const int n = first->count;
         u64 cut_key;
@@ -476,10 +488,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
             for (int bit = 63, turn = 0; bit >= 0; --bit, turn ^= 1) {
                 const u64 want = cut_key | 1ull << bit;
                 u64 own = 0;
-                for (int e = 0; e < count; ++e) {
-                    const float x = value(e);
+                each([&](float x, int e) {
                     if (member(x, e) && rank_key(x, r.index(e)) >= want) own += stage == 0 ? 1 : weight(x);
-                }
+                });
                 u64 sum;
                 block_scan(own, s.warp_sum, sum);
                 if (tid < blocks) cluster.map_shared_rank(&s, tid)->part[turn][me] = sum;
@@ -497,19 +508,26 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     }
 
     // ── the token ──
-    constexpr int kVec = Row<T>::kVec;
-    auto final_weight = [&](float x, int e) -> u32 {
-        if (!kept(x, e)) return 0;
-        const float w = weigh(x);
+    const bool cut = cut_x > -INFINITY;
+    auto final_weight = [&](float x, int i) -> u32 {   // i: the index
+        if (cut && !(x > cut_x || (x == cut_x && i <= cut_i))) return 0;
+        const float w = weigh.template weight<kUsual>(x);
         return w >= min_p ? whole(w) : 0;
     };
-    u64 mine = 0;
-    for (int e0 = 0; e0 < count; e0 += kVec) {
+    auto vector_sum = [&](int c) {
+        const uint4 raw = col[c * kThreads];
+        const T* y = reinterpret_cast<const T*>(&raw);
+        const int i = r.index(c * kVec);
         u64 own = 0;
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) own += final_weight(value(e0 + k), e0 + k);
-        own = warp_sum(own);
-        if (lane == 0) s.vec_sum[warp][e0 / kVec] = own;
+        for (int k = 0; k < kVec; ++k) own += final_weight(to_f32(y[k]), i + k);
+        return own;
+    };
+    u64 mine = 0;
+#pragma unroll 2
+    for (int c = 0; c < count / kVec; ++c) {
+        const u64 own = warp_sum(vector_sum(c));
+        if (lane == 0) s.vec_sum[warp][c] = own;
         mine += own;
     }
     __syncthreads();
@@ -536,15 +554,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     const u64 mark = mark_of(u, total);
     if (mark < before || mark >= before + mine) return;
     // this warp has it: its values in index order are (vector, lane, place)
-    int e = 0;
-    for (;; e += kVec) {
-        const u64 x = s.vec_sum[warp][e / kVec];
+    int c = 0;
+    for (;; ++c) {
+        const u64 x = s.vec_sum[warp][c];
         if (mark < before + x) break;
         before += x;
     }
-    u64 own = 0;
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) own += final_weight(value(e + k), e + k);
+    const u64 own = vector_sum(c);
     u64 upto = own;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -554,17 +570,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     const int src = __ffs(__ballot_sync(0xffffffffu, mark < before + upto)) - 1;
     before += __shfl_sync(0xffffffffu, upto - own, src);
     // that lane's vector, a value a lane
-    const int i = __shfl_sync(0xffffffffu, r.index(e), src) + lane;
-    float x = -INFINITY;
-    u32 w = 0;
-    if (lane < kVec) {
-        x = to_f32(col[(e + lane) * kThreads + (src - lane)]);
-        if (x > cut_x || (x == cut_x && i <= cut_i)) {
-            const float f = weigh(x);
-            w = f >= min_p ? whole(f) : 0;
-        }
-    }
-    upto = w;
+    const int i = __shfl_sync(0xffffffffu, r.index(c * kVec), src) + lane;
+    const float x = lane < kVec ? to_f32(reinterpret_cast<const T*>(col + c * kThreads + (src - lane))[lane]) : -INFINITY;
+    upto = lane < kVec ? final_weight(x, i) : 0;
 #pragma unroll
     for (int d = 1; d < kVec; d <<= 1) {
         const u64 y = __shfl_up_sync(0xffffffffu, upto, d);
@@ -572,6 +580,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     }
     const int at = __ffs(__ballot_sync(0xffffffffu, lane < kVec && mark < before + upto)) - 1;
     if (lane == at) write(i, (x == peak ? 0.f : weigh.power(x)) - log_weight(total));
+    };
+    if (weigh.usual())
+        rest(std::true_type{});
+    else
+        rest(std::false_type{});
 }
 
 // Values a thread: at most 32 of 32 bits or 64 of 16 (64 KB, two blocks an SM)
