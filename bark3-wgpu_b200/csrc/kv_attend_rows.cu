@@ -12,7 +12,7 @@
 // warp, so ragged batches and one long sequence keep every SM reading to the end.  A warp carries the
 // running maximum, sum and output of its item in registers; a run that covers
 // an item from end to end stores the result, other runs leave partial results
-// that k_join adds up in run order (same bits every time).
+// that k_attend_join adds up in run order (same bits every time).
 //
 // A step.  Each warp has its own ring of stages in shared memory, filled by
 // TMA boxes of a page's rows, lines of 128 bytes in the 128-byte swizzle.  Both
@@ -606,8 +606,9 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
 }
 
 // Adds up the partial results of the items that more than one run worked on,
-// a block an item, its warps shared out among the item's rows and of each row
-// among its runs.  Each lane keeps DIM / 32 channels.
+// a block an item (few items: a block an item and row), its warps shared out
+// among the rows and of each row among its runs.  Each lane keeps DIM / 32
+// channels.
 constexpr int kJoinMax = 32;   // warps
 
 template <typename T, int DIM, int ROWS>
@@ -630,10 +631,10 @@ __global__ void __launch_bounds__(kJoinMax * 32) k_attend_join(const __grid_cons
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int rows = sp.n * group;
-    const int share = max(1, warps / rows);        // warps a row
-    const int at_once = warps / share;             // rows at once
+    const int share = min(warps, max(1, warps * static_cast<int>(gridDim.y) / rows));   // warps a row
+    const int at_once = warps / share;                                                  // rows at once
     const float* ml = r.part + 2ll * r.workers * ROWS * DIM;
-    for (int row0 = 0; row0 < rows; row0 += at_once) {
+    for (int row0 = blockIdx.y * at_once; row0 < rows; row0 += at_once * gridDim.y) {
         const int row = row0 + warp / share, mine = warp % share;
         auto slot = [&](int w) { return (2ll * w + (w == w0 ? slot0 : 0)) * ROWS + row; };
         float m = -INFINITY, l = 0.f, o[kPer];
@@ -641,6 +642,7 @@ __global__ void __launch_bounds__(kJoinMax * 32) k_attend_join(const __grid_cons
         for (int i = 0; i < kPer; ++i) o[i] = 0.f;
         const bool live = row < rows && warp / share < at_once;
         if (live) {
+#pragma unroll 4
             for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, ml[slot(w) * 2]);
 #pragma unroll
             for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
@@ -705,8 +707,8 @@ int launch(const AttendParams& p, void* workspace, cudaStream_t st) {
     if (!rc) rc = make_map_2d(&mv, p.c.v, kMapU8, 128, lines, 128, 128, box, true);
     if (rc) return rc;
     RowsParams r{p, 0, 0, workers_of<DIM>(ROWS), ROWS, static_cast<float*>(workspace)};
-    // sequences a launch: the prefix array's room, and all their steps in 31 bits
-    const int64_t most = static_cast<int64_t>(p.b.table_width) * p.c.page_tokens / kStep + 1;
+    // sequences a launch: the prefix array's room, and all their units in 31 bits
+    const int64_t most = static_cast<int64_t>(p.b.table_width) * p.c.page_tokens / kStep + 2 + kItem;
     const int at_once = static_cast<int>(std::min<int64_t>(kMaxSeqs, 0x7fffffffll / most));
     for (; r.seq0 < p.b.n_seq; r.seq0 += at_once) {
         r.seqs = std::min(at_once, p.b.n_seq - r.seq0);
@@ -715,7 +717,7 @@ int launch(const AttendParams& p, void* workspace, cudaStream_t st) {
         if (e != cudaSuccess) return set_cuda_error("k_attend_rows", e);
         cudaLaunchConfig_t cfg = {};
         const int items = r.seqs * p.c.kv_heads;
-        cfg.gridDim = dim3(items);
+        cfg.gridDim = dim3(items, items * ROWS <= device_sms() ? ROWS : 1);
         // few items are cut into many runs each: more warps to read them
         cfg.blockDim = dim3(32 * (items > 4 * device_sms() ? 4 : items > device_sms() ? 8 : kJoinMax));
         cfg.stream = st;

@@ -503,10 +503,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                 if (!whole) {   // scores of keys that a row does not see become -inf in TMEM
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
+                        const int from = row_lo - key - 32 * c, to_ = row_hi - key - 32 * c;
+                        if (__all_sync(0xffffffffu, from <= 0 && to_ >= 32)) continue;
                         uint32_t a[32];
                         tmem_ld_32x32b_x32(ts + 32 * c, a);
                         tmem_wait_ld();
-                        const int from = row_lo - key - 32 * c, to_ = row_hi - key - 32 * c;
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (i < from || i >= to_) a[i] = 0xff800000u;

@@ -13,8 +13,7 @@
 // by it alone; a warp's values are neighbours in the row, in index order over
 // (vector, lane, place)).  Shared memory and not registers: loops over 32
 // values unrolled with an exponential in each miss the instruction cache.
-// Bound by the instructions of some thirty operations a value for many rows,
-// by the chain of block- and cluster-wide steps for few.
+// Bound by some fifty instructions a value for many rows, by the chain of block- and cluster-wide steps for few.
 //   top_k <= 512   Each warp's j-th largest thread maximum, j = ceil(k / warps),
 //                  bounds the k-th largest logit from below (the warps hold k
 //                  values that large); what reaches the bound, a few hundred

@@ -257,8 +257,9 @@ int b3_attn_conv(b3_ctx* ctx, int layer, float* x, int t, unsigned flags);
  * default stream), nothing is allocated and nothing waits, so the calls can
  * be captured in a CUDA graph.  Arguments that the host can see are checked
  * before anything is launched (B3_EINVAL).  Lengths and page numbers live on
- * the device; a kernel that meets one out of range skips that access and sets
- * a B3_KV_BAD_* bit in the cache's status word.
+ * the device; a kernel that meets one out of range keeps clear of it, sets a
+ * B3_KV_BAD_* bit in the cache's status word and goes on (what it concerns is
+ * not written, or holds no meaning).
  *
  * The cache holds 8-bit floats (e4m3: 4 exponent and 3 mantissa bits, largest
  * 448) and a scale for each page and head that is a power of two:
