@@ -217,7 +217,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // Barriers.  k, v: two stages each, phases over the CTA's blocks; q: a half's
     // queries are staged (an item); s: a half's scores are in TMEM, p: its
-    // probabilities are (a block); o: its last product is done (an item).
+    // probabilities of the first 64 keys, and of all, are (a block; PV starts on
+    // the first while the softmax is at the rest); o: its last product is done
+    // (an item).
     const uint32_t bars = smem_u32(smem + C::kBar);
     auto k_full = [&](int s) { return bars + 8 * s; };
     auto k_empty = [&](int s) { return bars + 16 + 8 * s; };
@@ -225,9 +227,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
     auto v_empty = [&](int s) { return bars + 48 + 8 * s; };
     auto q_full = [&](int h) { return bars + 64 + 8 * h; };
     auto s_full = [&](int h) { return bars + 80 + 8 * h; };
-    auto p_full = [&](int h) { return bars + 96 + 8 * h; };
-    auto o_full = [&](int h) { return bars + 112 + 8 * h; };
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBar + 128);
+    auto p_half = [&](int h) { return bars + 96 + 8 * h; };
+    auto p_full = [&](int h) { return bars + 112 + 8 * h; };
+    auto o_full = [&](int h) { return bars + 128 + 8 * h; };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBar + 160);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full(i), 8);
@@ -236,6 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
             mbar_init(v_empty(i), 1);
             mbar_init(q_full(i), 4);
             mbar_init(s_full(i), 1);
+            mbar_init(p_half(i), 4);
             mbar_init(p_full(i), 4);
             mbar_init(o_full(i), 1);
         }
@@ -289,16 +293,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                 for (int j = 0; j < n && ok; ++j, ++g) {
                     const uint32_t st = g & 1;
                     for (int h = 0; h < nh && ok; ++h) {
-                        ok = mbar_wait(p_full(h), blocks[h] & 1, 0x72);
-                        ++blocks[h];
-                        if (ok && h == 0) ok = mbar_wait(v_full(st), (g >> 1) & 1, 0x73);
-                        if (!ok) break;
-                        tc_fence_after();
                         const uint64_t bv = smem_desc_sw128_mn(sv + st * C::kOperand, C::kHalf, 1024);
+                        for (int part = 0; part < 2 && ok; ++part) {   // 64 keys each
+                            ok = mbar_wait(part ? p_full(h) : p_half(h), blocks[h] & 1, 0x72);
+                            if (ok && h == 0 && part == 0) ok = mbar_wait(v_full(st), (g >> 1) & 1, 0x73);
+                            if (!ok) break;
+                            tc_fence_after();
 #pragma unroll
-                        for (int k = 0; k < kKeys / 16; ++k)
-                            mma_f16_ts(tmem + C::kTmemO + 128 * h, tmem + C::kTmemS + 128 * h + 8 * k, desc_advance(bv, 2048 * k),
-                                       C::kIdescPV, j > 0 || k > 0);
+                            for (int k = 0; k < 4; ++k)
+                                mma_f16_ts(tmem + C::kTmemO + 128 * h, tmem + C::kTmemS + 128 * h + 32 * part + 8 * k,
+                                           desc_advance(bv, 8192 * part + 2048 * k), C::kIdescPV, j > 0 || part > 0 || k > 0);
+                        }
+                        if (!ok) break;
+                        ++blocks[h];
                         if (h == nh - 1) mma_commit(v_empty(st));
                         if (j == n - 1) mma_commit(o_full(h));
                         if (j + 1 < n) {
@@ -579,6 +586,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                         l = fmaf(sum.x + sum.y, exp2_int(-ei), l);
                     }
                     tmem_st_32x32b_x16(ts + 16 * c, b);   // over scores that were read
+                    if (c == 1) {                         // the first 64 keys' probabilities are there
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_half(h));
+                    }
                 }
                 tmem_wait_st();
                 tc_fence_before();
