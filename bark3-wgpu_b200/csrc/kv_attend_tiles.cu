@@ -32,6 +32,12 @@
 // cut into equal runs, one a CTA, so causal triangles, ragged prompts and few
 // rows over many keys end together.  A run that covers an item from end to end stores it, other runs
 // leave partial results that k_attend_tiles_join adds up in run order.
+//
+// Measured: 2048 tokens over 16384, 32 query and 8 key heads of 128, 583 us
+// (884 TFLOP/s).  The chain softmax, PV, S of a half sets the pace: a half's
+// softmax takes 3600 cycles a block beside the other half's, PV and S 1240.
+// Reading the scores twice (593 us then) beat reading them once (794), two
+// threads a row (648), exponentials by groups of 16 keys (619), 64-key blocks (713).
 #include <type_traits>
 
 #include "b3_ptx.cuh"

@@ -13,7 +13,9 @@
 // by it alone; a warp's values are neighbours in the row, in index order over
 // (vector, lane, place)).  Shared memory and not registers: loops over 32
 // values unrolled with an exponential in each miss the instruction cache.
-// Bound by some fifty instructions a value for many rows, by the chain of block- and cluster-wide steps for few.
+// Bound by some 57 instructions a value for many rows, by the chain of block-
+// and cluster-wide steps for few.  Measured, settings of each kind mixed: 256 rows
+// x 131072 in 16 bits 124 us (one read takes 10), 256 x 8193 in f32 24, one row 11.
 //   top_k <= 512   Each warp's j-th largest thread maximum, j = ceil(k / warps),
 //                  bounds the k-th largest logit from below (the warps hold k
 //                  values that large); what reaches the bound, a few hundred
@@ -588,7 +590,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
 
 // Values a thread: at most 32 of 32 bits or 64 of 16 (64 KB, two blocks an SM)
 // where the row fits a cluster so.  Fewer, longer blocks are better than more:
-// 256 rows x 131072 in 16 bits with top_k 94 us in clusters of four, 162 of eight.
+// 256 rows x 131072 in 16 bits with top_k 94 us in clusters of four, 162 of eight
+// (with every value divided by the temperature, as unusual rows still are).
 template <typename T>
 int launch(const b3_sample_args& a, cudaStream_t st) {
     constexpr int kVec = Row<T>::kVec;
