@@ -218,6 +218,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     const cg::cluster_group cluster = cg::this_cluster();
     const int blocks = cluster.num_blocks(), me = cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / blocks;
+    if (blocks > 1) cluster.barrier_arrive();   // this block runs: its shared memory may be written from outside
     Shared* const first = cluster.map_shared_rank(&s, 0);
     constexpr int kVec = Row<T>::kVec;
     uint4* const col = values + tid;      // vector c of the thread at col[c * kThreads]
@@ -282,6 +283,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     }
     if (j > 32) jth = -INFINITY;
     if (blocks > 1) {
+        cluster.barrier_wait();   // every block of the cluster runs; reached behind the row's loads, so long since done
         if (tid < blocks) {
             Shared* const to = cluster.map_shared_rank(&s, tid);
             to->peak[me] = peak;
