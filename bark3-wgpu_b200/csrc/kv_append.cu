@@ -464,7 +464,7 @@ int kv_check(const b3_kv_cache* c, const b3_kv_batch* b) {
                          c->kv_heads, c->page_tokens);
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
         return set_error(B3_EINVAL, "the cache's codes must be 16-byte aligned");
-    if (b->n_seq <= 0 || b->tokens < 0 || b->table_width <= 0 || b->table_stride < b->table_width)
+    if (b->n_seq <= 0 || b->tokens < 0 || b->table_width <= 0 || (b->table_stride < b->table_width && b->table_stride != 0))
         return set_error(B3_EINVAL, "batch of %d sequences, %d tokens, page table %d wide with stride %lld", b->n_seq,
                          b->tokens, b->table_width, static_cast<long long>(b->table_stride));
     if (static_cast<int64_t>(b->table_width) * c->page_tokens > 0x7fffffffll)

@@ -642,7 +642,7 @@ extern "C" int b3_sample(const b3_sample_args* args, void* stream) {
     const b3_sample_args& a = *args;
     if (a.rows == 0) return 0;
     if (!a.logits || !a.uniform || !a.ids) return set_error(B3_EINVAL, "null logits, uniform or ids");
-    if (a.rows < 0 || a.vocab <= 0 || a.vocab > B3_SAMPLE_MAX_VOCAB || a.row_stride < a.vocab)
+    if (a.rows < 0 || a.vocab <= 0 || a.vocab > B3_SAMPLE_MAX_VOCAB || (a.row_stride < a.vocab && a.row_stride != 0))
         return set_error(B3_EINVAL, "logits of %d rows x %d (at most %d), row stride %lld", a.rows, a.vocab,
                          B3_SAMPLE_MAX_VOCAB, static_cast<long long>(a.row_stride));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -94,6 +94,10 @@ at::Tensor output(PyObject* o, at::IntArrayRef shape, const at::Tensor& like, at
     return t;
 }
 
+// Elements from row to row of a tensor with adjacent columns.  That of a single row is any number in torch;
+// 0 (an expanded tensor: every row the same) and what else there is goes to the ABI's checks.
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
 int i32(int64_t v, const char* name) {
     if (v < 0 || v > 0x7fffffff) raise(B3_EINVAL, std::string(name) + " " + std::to_string(v) + " is out of range");
     return static_cast<int>(v);
@@ -140,7 +144,7 @@ b3_kv_batch batch(const Cache* self, int64_t tokens, PyObject* cu_q, PyObject* k
                              describe(table));
     b.page_table = static_cast<const int32_t*>(table.data_ptr());
     b.table_width = i32(table.size(1), "page_table's width");
-    b.table_stride = std::max(table.stride(0), table.size(1));
+    b.table_stride = row_stride(table);
     b.n_seq = i32(n, "the number of sequences");
     b.tokens = i32(tokens, "the number of tokens");
     return b;
@@ -319,7 +323,7 @@ PyObject* sample(PyObject*, PyObject* args, PyObject* kwargs) {
         a.min_p = vector<float>(m, "min_p", at::kFloat, n, device);
         a.rows = i32(n, "the number of rows");
         a.vocab = i32(x.size(1), "the vocabulary");
-        a.row_stride = std::max(x.stride(0), x.size(1));
+        a.row_stride = row_stride(x);
         at::Tensor ids = at::empty({n}, x.options().dtype(at::kInt)), logprob = at::empty({n}, x.options().dtype(at::kFloat));
         a.ids = static_cast<int32_t*>(ids.data_ptr());
         a.logprob = static_cast<float*>(logprob.data_ptr());

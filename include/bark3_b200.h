@@ -292,12 +292,13 @@ typedef struct b3_kv_cache {
  * cu_q[i] .. cu_q[i+1], which are the last of its kv_lens[i] tokens; token j
  * of it lives in slot j % page_tokens of page page_table[i][j / page_tokens].
  * Table entries past the last token are never read.  A sequence may have no
- * new tokens, or (attention only) no tokens at all. */
+ * new tokens, or (attention only) no tokens at all.  Sequences may share pages
+ * that are only read; a page that receives tokens belongs to one of them. */
 typedef struct b3_kv_batch {
     const int32_t* cu_q;        /* [n_seq + 1], cu_q[0] = 0, cu_q[n_seq] = tokens */
     const int32_t* kv_lens;     /* [n_seq], the new tokens included */
     const int32_t* page_table;  /* [n_seq][table_stride], table_width entries in use */
-    int64_t table_stride;
+    int64_t table_stride;       /* at least table_width, or 0: one row for all sequences */
     int32_t table_width;
     int32_t n_seq;
     int32_t tokens;
@@ -381,7 +382,7 @@ typedef struct b3_sample_args {
     const float* min_p;        /* [rows] or NULL; <= 0: off */
     int32_t* ids;              /* [rows] */
     float* logprob;            /* [rows] or NULL */
-    int64_t row_stride;
+    int64_t row_stride;        /* at least vocab, or 0: one row of logits for all */
     int32_t dtype;             /* B3_DTYPE_F32, F16 or BF16 */
     int32_t rows;
     int32_t vocab;             /* at most B3_SAMPLE_MAX_VOCAB */
