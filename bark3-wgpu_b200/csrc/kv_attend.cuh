@@ -73,50 +73,74 @@ __device__ __forceinline__ void seen_keys(const AttendParams& p, const SeqSpan& 
     }
 }
 
-// One query row by one warp in plain arithmetic, a key at a time: the keys of
-// [k0, k1) that the row sees, m in the units above, o and l against it, o in
-// DIM / 32 channels a lane.  A masked key does not touch the row, whatever it
-// holds; in the tensor cores' sums 0 * NaN of a value that other rows see is
-// NaN, so rows whose output came out NaN are taken again by this.
-template <typename T, int DIM>
-__device__ __noinline__ void attend_row_exact(const AttendParams& p, int seq, int token, int i, int q_head, int k0, int k1,
-                                              float (&o)[DIM / 32], float& m, float& l) {
-    constexpr int kPer = DIM / 32;
-    const int lane = threadIdx.x & 31, page = p.c.page_tokens, kv_head = q_head / (p.a.q_heads / p.c.kv_heads);
-    const SeqSpan sp = attend_span(p, seq);
-    int lo, hi;
-    seen_keys(p, sp, i, lo, hi);
-    const T* q = static_cast<const T*>(p.a.q) + token * p.a.q_token_stride + q_head * p.a.q_head_stride + lane * kPer;
-    float x[kPer];
-    for (int c = 0; c < kPer; ++c) {
-        x[c] = to_f32(q[c]) * (p.a.scale * kLog2e);
-        o[c] = 0.f;
+// What the new tokens i0 .. i1 of a sequence see together: each key of
+// [any_lo, any_hi) some of them, each of [lo_max, hi_min) all of them.
+struct SeenByRows {
+    int any_lo, lo_max, hi_min, any_hi;
+    __device__ __forceinline__ bool whole(int key, int n) const { return key >= lo_max && key + n <= hi_min; }
+    // keys [key, key + n) that not all rows see, where rows see different keys at all
+    __device__ __forceinline__ bool split(int key, int n) const {
+        return (any_lo != lo_max || any_hi != hi_min) && !whole(key, n);
     }
-    m = -INFINITY;
-    l = 0.f;
-    for (int j = max(lo, k0); j < min(hi, k1); ++j) {
-        int id = __ldg(p.b.page_table + seq * p.b.table_stride + j / page);
-        if (id < 0 || id >= p.c.pages) id = 0;   // flagged where it was met first
-        const int64_t slab = static_cast<int64_t>(id) * p.c.kv_heads + kv_head;
-        const int64_t at = (slab * page + j % page) * DIM + lane * kPer;
-        float dot = 0.f;
-        for (int c = 0; c < kPer; c += 2) {
-            const float2 k = __half22float2(decode2(*reinterpret_cast<const uint16_t*>(p.c.k + at + c)));
-            dot = fmaf(x[c], k.x, fmaf(x[c + 1], k.y, dot));
+};
+__device__ __forceinline__ SeenByRows seen_by_rows(const AttendParams& p, const SeqSpan& s, int i0, int i1) {
+    SeenByRows r;
+    seen_keys(p, s, i0, r.any_lo, r.hi_min);
+    seen_keys(p, s, i1, r.lo_max, r.any_hi);
+    return r;
+}
+
+// NaN values.  In the tensor cores' sums 0 * NaN of a value that a row does not
+// see would be NaN, so in blocks of keys that only some rows see (SeenByRows::
+// split) NaN codes of V go into the product as 0, and the rows that do see them
+// get their NaN back at the end, by nan_channels over those blocks: their
+// number depends on the rows of a tile, not on the length of the sequence.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t four) {   // bit 7 of each byte that is an e4m3 NaN
+    return ((four & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+__device__ __forceinline__ uint32_t without_codes(uint32_t four, uint32_t nans) { return four & ~((nans >> 7) * 0xffu); }
+
+// By a whole warp; each lane has a row that sees the keys [lo, hi).  Sets bit b
+// of mask[c] where one of these among [k0, k1) holds NaN in channel
+// b * (DIM / 32) + c of V.
+template <int DIM>
+__device__ __noinline__ void nan_channels(const AttendParams& p, int seq, int kv_head, int k0, int k1, int lo, int hi,
+                                          uint32_t (&mask)[DIM / 32]) {
+    constexpr int kPer = DIM / 32, kAhead = 4;
+    const int lane = threadIdx.x & 31, page = p.c.page_tokens;
+    for (int j0 = k0; j0 < k1; j0 += kAhead) {
+        uint32_t nans[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int j = j0 + i;
+            uint32_t w = 0;
+            if (j < k1) {
+                int id = __ldg(p.b.page_table + seq * p.b.table_stride + j / page);
+                if (id < 0 || id >= p.c.pages) id = 0;   // flagged where it was met first
+                const uint8_t* v = p.c.v + ((static_cast<int64_t>(id) * p.c.kv_heads + kv_head) * page + j % page) * DIM + lane * kPer;
+                w = kPer == 4 ? *reinterpret_cast<const uint32_t*>(v) : *reinterpret_cast<const uint16_t*>(v);
+            }
+            nans[i] = nan_codes(w);
         }
-        for (int w = 16; w; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
-        const int ve = stored_exp(p.c.v_scale[slab]);
-        dot = fmaf(dot, p.c.k_scale[slab], static_cast<float>(ve));
-        const float top = fmaxf(m, dot), ref = top == -INFINITY ? 0.f : top;
-        const float old = m == top ? 1.f : ex2_approx(m - top), e = ex2_approx(dot - ref);
-        l = fmaf(e, exp2_int(-ve), l * old);
-        for (int c = 0; c < kPer; c += 2) {
-            const float2 v = __half22float2(decode2(*reinterpret_cast<const uint16_t*>(p.c.v + at + c)));
-            o[c] = fmaf(e, v.x, o[c] * old);
-            o[c + 1] = fmaf(e, v.y, o[c + 1] * old);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (!__any_sync(0xffffffffu, nans[i])) continue;
+            const bool sees = j0 + i >= lo && j0 + i < hi;
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) {
+                const uint32_t m = __ballot_sync(0xffffffffu, nans[i] >> (8 * c + 7) & 1);
+                if (sees) mask[c] |= m;
+            }
         }
-        m = top;
     }
+}
+
+// NaN into the channels of mask of a row at `out`.
+template <int DIM, typename U>
+__device__ __forceinline__ void put_nan(U* out, const uint32_t (&mask)[DIM / 32]) {
+#pragma unroll
+    for (int c = 0; c < DIM / 32; ++c)
+        for (uint32_t m = mask[c]; m; m &= m - 1) from_f32(__uint_as_float(0x7fffffffu), out[(__ffs(m) - 1) * (DIM / 32) + c]);
 }
 
 // The float of a finished row: o / l, zeros where nothing was seen.

@@ -190,6 +190,45 @@ __device__ __forceinline__ void store_row(const AttendParams& p, int token, int 
     }
 }
 
+// NaN codes out of a staged V of `bytes`, by a warp; true if this lane met one.
+// Out of line: few steps need it, and in line the compiler predicates it.
+__device__ __noinline__ bool clean_v(uint32_t v, uint32_t bytes) {
+    uint32_t any = 0;
+    for (uint32_t at = v + 16 * (threadIdx.x & 31); at < v + bytes; at += 512) {
+        const uint4 x = lds128(at), n = make_uint4(nan_codes(x.x), nan_codes(x.y), nan_codes(x.z), nan_codes(x.w));
+        if (!(n.x | n.y | n.z | n.w)) continue;
+        any = 1;
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(without_codes(x.x, n.x)),
+                     "r"(without_codes(x.y, n.y)), "r"(without_codes(x.z, n.z)), "r"(without_codes(x.w, n.w))
+                     : "memory");
+    }
+    if (any) fence_async_shared();   // the next TMA box into this stage comes after these stores
+    return any;
+}
+
+// NaN back into the rows of an item, where a key of [key0, key1) that the row
+// sees holds it; lane i has row i.  The rows have been stored, by all lanes, as
+// output (slot < 0) or partial results.
+template <typename T, int DIM, int ROWS>
+__device__ __noinline__ void restore_nan(const RowsParams& r, int seq, int head, int key0, int key1, int64_t slot) {
+    const AttendParams& p = r.p;
+    const SeqSpan sp = attend_span(p, seq);
+    const SeenByRows see = seen_by_rows(p, sp, 0, sp.n - 1);
+    const int lane = threadIdx.x & 31, group = p.a.q_heads / p.c.kv_heads;
+    const bool live = lane < sp.n * group;
+    uint32_t mask[DIM / 32] = {};
+    int lo = 0, hi = 0;
+    if (live) seen_keys(p, sp, lane / group, lo, hi);
+    for (int key = key0; key < key1; key += kStep)
+        if (see.split(key, kStep)) nan_channels<DIM>(p, seq, head, max(key, see.any_lo), min(key + kStep, key1), lo, hi, mask);
+    __syncwarp();
+    if (live && slot < 0)
+        put_nan<DIM>(static_cast<T*>(p.a.out) +
+                         (static_cast<int64_t>(sp.first + lane / group) * p.a.q_heads + head * group + lane % group) * DIM, mask);
+    else if (live)
+        put_nan<DIM>(r.part + (slot * ROWS + lane) * DIM, mask);
+}
+
 template <typename T, int DIM, int ROWS>
 __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
     k_attend_rows(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -358,10 +397,8 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
                 seen_keys(p, sp, mine < n_rows ? mine / group : 0, row_lo[hf][e], row_hi[hf][e]);
             }
         }
-        // keys that every row sees: [lo_max, hi_min), that some row sees: [any_lo, any_hi)
-        int lo_max, hi_min, any_lo, any_hi;
-        seen_keys(p, sp, 0, any_lo, hi_min);
-        seen_keys(p, sp, sp.n - 1, lo_max, any_hi);
+        const SeenByRows see = seen_by_rows(p, sp, 0, sp.n - 1);
+        bool nans = false;   // this lane has taken NaN codes of V out
 
         float o[kHalves][kSteps][4], m[kHalves][2], l[kHalves][2];
 #pragma unroll
@@ -435,7 +472,7 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
                     }
                 }
             }
-            const bool whole = key >= lo_max && key + kStep <= hi_min;   // no row masks any key here
+            const bool whole = see.whole(key, kStep);   // no row masks any key here
             float top[kHalves][2];
 #pragma unroll
             for (int hf = 0; hf < kHalves; ++hf)
@@ -503,6 +540,10 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
             }
 
             // ── output ──
+            if (see.split(key, kStep)) {
+                nans |= clean_v(vbase, C::kHalf);
+                __syncwarp();
+            }
 #pragma unroll
             for (int mt = 0; mt < kTilesM; ++mt) {
                 uint32_t w[4][DIM / 32];
@@ -519,7 +560,7 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
                         w[i][0] = q2.x, w[i][1] = q2.y;
                     }
                     // a key that no row sees may hold anything, NaN codes among it: 0 * NaN is no zero
-                    if (!whole && (key + kk < any_lo || key + kk >= any_hi))
+                    if (!whole && (key + kk < see.any_lo || key + kk >= see.any_hi))
 #pragma unroll
                         for (int j = 0; j < DIM / 32; ++j) w[i][j] = 0;
                 }
@@ -572,41 +613,7 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
                 }
             }
         if (!ok) break;
-        if (sp.n > 1 && p.a.causal) {
-            // rows that came out NaN (or infinite), where rows see different keys: again, without the keys they do not see
-            __syncwarp();
-#pragma unroll
-            for (int hf = 0; hf < kHalves; ++hf)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float nan = 0.f;
-#pragma unroll
-                    for (int j = 0; j < kSteps; ++j) nan = fmaf(o[hf][j][e], 0.f, fmaf(o[hf][j][2 + e], 0.f, nan));
-                    const unsigned bad = __ballot_sync(0xffffffffu, nan != nan);   // lane 4 g + t: a part of row 2 t + e
-                    for (int c = 0; c < 4; ++c) {
-                        const int row = 2 * c + e + 8 * hf;
-                        if (!(bad & (0x11111111u << c)) || row >= n_rows) continue;
-                        const int i = row / group, head = it.head * group + row % group;
-                        float x[DIM / 32], mm, ll;
-                        attend_row_exact<T, DIM>(p, seq, sp.first + i, i, head, key0, key1, x, mm, ll);
-                        const int64_t out = static_cast<int64_t>(sp.first + i) * p.a.q_heads + head;
-                        for (int d = 0; d < DIM / 32; ++d) {
-                            const int ch = lane * (DIM / 32) + d;
-                            if (all)
-                                from_f32(x[d] * row_inverse(ll), static_cast<T*>(p.a.out)[out * DIM + ch]);
-                            else
-                                r.part[(slot * ROWS + row) * DIM + ch] = x[d];
-                        }
-                        if (lane == 0) {
-                            if (!all)
-                                *reinterpret_cast<float2*>(r.part + 2ll * r.workers * ROWS * DIM + (slot * ROWS + row) * 2) =
-                                    make_float2(mm, ll);
-                            else if (p.a.lse)
-                                p.a.lse[out] = row_lse(mm, ll);
-                        }
-                    }
-                }
-        }
+        if (__any_sync(0xffffffffu, nans)) restore_nan<T, DIM, ROWS>(r, seq, it.head, key0, key1, all ? -1 : slot);
     }
 }
 

@@ -214,6 +214,55 @@ __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+    return x;
+}
+
+// NaN out of the f16 values that a lane has staged of a task of V: LOADS times
+// 16 channels of every KEYS-th key; sets *seen if there was one.  Out of line:
+// in line the compiler predicates it, and every task pays (2048 tokens over
+// 16384 660 us instead of 595).
+template <int LOADS, int KEYS>
+__device__ __noinline__ void clean_v(uint32_t to, int sub, int c0, volatile uint32_t* seen) {
+#pragma unroll 1
+    for (int i = 0; i < 2 * LOADS; ++i) {
+        const uint32_t at = to + (i >> 1) * KEYS * 128 + (((c0 + (i & 1)) ^ ((sub + (i >> 1) * KEYS) & 7)) << 4);
+        uint4 x = lds128(at);
+        auto nan = [](uint32_t two) { return ((two & 0x7fff7fffu) + 0x03ff03ffu) & 0x80008000u; };   // bit 15 of a half that is NaN
+        const uint4 n = make_uint4(nan(x.x), nan(x.y), nan(x.z), nan(x.w));
+        if (!(n.x | n.y | n.z | n.w)) continue;
+        *seen = 1;
+        sts128(at, x.x & ~((n.x >> 15) * 0xffffu), x.y & ~((n.y >> 15) * 0xffffu), x.z & ~((n.z >> 15) * 0xffffu),
+               x.w & ~((n.w >> 15) * 0xffffu));
+    }
+}
+
+// NaN back into row i of an item, where a key of the blocks [s0, s1) that the
+// row sees holds it; a row a lane.  The row has been stored as output (slot < 0)
+// or partial result.
+template <typename T, int DIM>
+__device__ __noinline__ void restore_nan(const TilesParams& r, const Tile& t, int head, int s0, int s1, int i, bool live, int64_t slot) {
+    const AttendParams& p = r.p;
+    const int group = p.a.q_heads / p.c.kv_heads, last = min(t.row0 + kRows, t.n * group) - 1, row = min(t.row0 + i, last);
+    const SeqSpan sp = {t.first, t.n, t.len};
+    const SeenByRows see = seen_by_rows(p, sp, t.row0 / group, last / group);
+    int lo, hi;
+    seen_keys(p, sp, row / group, lo, hi);
+    uint32_t mask[DIM / 32] = {};
+    for (int j = s0; j < s1; ++j) {
+        const int key = t.key_lo + j * kKeys;
+        if (see.split(key, kKeys))
+            nan_channels<DIM>(p, t.seq, head, max(key, see.any_lo), min(key + kKeys, see.any_hi), lo, hi, mask);
+    }
+    if (live && slot < 0)
+        put_nan<DIM>(static_cast<T*>(p.a.out) +
+                         (static_cast<int64_t>(t.first + row / group) * p.a.q_heads + head * group + row % group) * DIM, mask);
+    else if (live)
+        put_nan<DIM>(r.part + (slot * kRows + i) * DIM, mask);
+}
+
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_constant__ TilesParams r) {
     using C = Cfg<DIM>;
@@ -237,7 +286,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
     auto p_full = [&](int h) { return bars + 112 + 8 * h; };
     auto o_full = [&](int h) { return bars + 128 + 8 * h; };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBar + 160);
+    // set when NaN codes of V have gone into a product as 0: before v_full of their block, read behind o_full
+    volatile uint32_t* nan_seen = reinterpret_cast<uint32_t*>(smem + C::kBar + 164);
     if (threadIdx.x == 0) {
+        *nan_seen = 0;
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full(i), 8);
             mbar_init(v_full(i), 8);
@@ -342,19 +394,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
         const uint32_t dst = smem_u32(smem) + (piece >> 2) * C::kHalf + sub * 128;
         const int c0 = 2 * (piece & 3);
         uint32_t block = 0;
-        int any_lo, any_hi;                  // keys that some row of the item sees; block of the run the loads are at
+        // of the item that the loads are at: keys that some row sees; its blocks before and from which rows see
+        // different keys (SeenByRows::split)
+        int any_lo, any_hi, split_lo, split_hi;
         const int32_t* pages;
         auto item = [&]() {
             const SeqSpan sp = {w.t.first, w.t.n, w.t.len};
-            const int last = min(w.t.row0 + kRows, w.t.n * group) - 1;
-            int x;
-            seen_keys(p, sp, w.t.row0 / group, any_lo, x);
-            seen_keys(p, sp, last / group, x, any_hi);
+            const SeenByRows see = seen_by_rows(p, sp, w.t.row0 / group, (min(w.t.row0 + kRows, w.t.n * group) - 1) / group);
+            any_lo = see.any_lo, any_hi = see.any_hi;
+            const bool differ = see.split(see.hi_min, kKeys);
+            split_lo = differ ? (see.lo_max - w.t.key_lo + kKeys - 1) / kKeys : 0;
+            split_hi = differ ? (see.hi_min - w.t.key_lo) / kKeys : 0x7fffffff;
             pages = p.b.page_table + w.t.seq * p.b.table_stride;
         };
         item();
         bool more = true;
-        auto fetch = [&](uint32_t q, uint4 (&c)[kLoads]) {   // false where the run has no such task
+        enum { kNone, kPlain, kSplitV };
+        auto fetch = [&](uint32_t q, uint4 (&c)[kLoads]) -> int {   // kNone where the run has no such task
             if ((q >> 4) != block && more) {
                 ++block;
                 if (++w.s0 == w.s1) {
@@ -362,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                     if (more) item();
                 }
             }
-            if (!more) return false;
+            if (!more) return kNone;
             const int key = w.t.key_lo + w.s0 * kKeys + 16 * (q & 7);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) c[i] = make_uint4(0, 0, 0, 0);   // a key that no row sees: 0, whatever its place holds
@@ -380,9 +436,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                     if (k >= any_lo && k < any_hi) c[i] = __ldg(reinterpret_cast<const uint4*>(from + i * kKeysLoad * DIM));
                 }
             }
-            return true;
+            return (q & 8) && (w.s0 < split_lo || w.s0 >= split_hi) ? kSplitV : kPlain;
         };
-        auto expand = [&](uint32_t q, const uint4 (&c)[kLoads]) {
+        auto expand = [&](uint32_t q, const uint4 (&c)[kLoads], int kind) {
             const uint32_t g = q >> 4, st = g & 1, v = (q >> 3) & 1, key = 16 * (q & 7);
             if (g >= 2) ok = __all_sync(0xffffffffu, mbar_wait(v ? v_empty(st) : k_empty(st), ((g >> 1) - 1) & 1, 0x75));
             if (!ok) return;
@@ -401,20 +457,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                 sts128(to + i * kKeysLoad * 128 + ((c0 ^ sw) << 4), out[0], out[1], out[2], out[3]);
                 sts128(to + i * kKeysLoad * 128 + (((c0 + 1) ^ sw) << 4), out[4], out[5], out[6], out[7]);
             }
+            if (kind == kSplitV) clean_v<kLoads, kKeysLoad>(to, sub, c0, nan_seen);
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(v ? v_full(st) : k_full(st));
         };
         uint4 ca[kLoads], cb[kLoads];
         const uint32_t first = warp - kExpWarp0;
-        bool has_a = fetch(first, ca), has_b = has_a && fetch(first + kExpWarps, cb);
-        for (uint32_t q = first; has_a && ok; q += 2 * kExpWarps) {
-            expand(q, ca);
-            if (!ok || !has_b) break;
-            has_a = fetch(q + 2 * kExpWarps, ca);
-            expand(q + kExpWarps, cb);
+        int a = fetch(first, ca), b = a != kNone ? fetch(first + kExpWarps, cb) : kNone;
+        for (uint32_t q = first; a != kNone && ok; q += 2 * kExpWarps) {
+            expand(q, ca, a);
+            if (!ok || b == kNone) break;
+            a = fetch(q + 2 * kExpWarps, ca);
+            expand(q + kExpWarps, cb, b);
             if (!ok) break;
-            has_b = has_a && fetch(q + 3 * kExpWarps, cb);
+            b = a != kNone ? fetch(q + 3 * kExpWarps, cb) : kNone;
         }
         if (!ok && lane == 0) kv_flag(p.c.status, B3_KV_TIMEOUT);
     } else {
@@ -478,11 +535,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
             const SeqSpan sp = {t.first, t.n, t.len};
             const int rows = min(128, t.n * group - t.row0 - 128 * h);
             const int row = t.row0 + 128 * h + min(mine, rows - 1);
-            int row_lo, row_hi, lo_max, hi_min, x;
+            int row_lo, row_hi, any_lo, any_hi, x;
             seen_keys(p, sp, row / group, row_lo, row_hi);
-            seen_keys(p, sp, (t.row0 + 128 * h) / group, x, hi_min);
-            seen_keys(p, sp, (t.row0 + 128 * h + rows - 1) / group, lo_max, x);
-            int any_lo, any_hi;
+            const SeenByRows half = seen_by_rows(p, sp, (t.row0 + 128 * h) / group, (t.row0 + 128 * h + rows - 1) / group);
             seen_keys(p, sp, t.row0 / group, any_lo, x);
             seen_keys(p, sp, (min(t.row0 + kRows, t.n * group) - 1) / group, x, any_hi);
             const int32_t* pages = p.b.page_table + t.seq * p.b.table_stride;
@@ -512,8 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                 if (!ok) break;
                 tc_fence_after();
                 const int key = t.key_lo + j * kKeys;
-                const bool whole = key >= lo_max && key + kKeys <= hi_min;
-                if (!whole) {   // scores of keys that a row does not see become -inf in TMEM
+                if (!half.whole(key, kKeys)) {   // scores of keys that a row does not see become -inf in TMEM
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         const int from = row_lo - key - 32 * c, to_ = row_hi - key - 32 * c;
@@ -620,14 +674,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
             T* out = static_cast<T*>(p.a.out) + (static_cast<int64_t>(token) * p.a.q_heads + q_head) * DIM;
             float* po = r.part + (slot * kRows + 128 * h + mine) * DIM;
             float* ml = r.part + 2ll * r.runs * kRows * DIM + (slot * kRows + 128 * h + mine) * 2;
-            float nan = 0.f;
 #pragma unroll
             for (int c = 0; c < DIM / 32; ++c) {
                 uint32_t a[32];
                 tmem_ld_32x32b_x32(to + 32 * c, a);
                 tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) nan = fmaf(__uint_as_float(a[i]), 0.f, nan);
                 if (live && all) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
@@ -648,27 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
             } else if (live) {
                 *reinterpret_cast<float2*>(ml) = make_float2(m, l);
             }
-            // rows that came out NaN (or infinite): again, without the keys they do not see
-            unsigned bad = __ballot_sync(0xffffffffu, live && nan != nan);
-            while (bad) {
-                const int src = __ffs(bad) - 1;
-                bad &= bad - 1;
-                const int rr = t.row0 + 128 * h + (warp & 3) * 32 + src;
-                const int tok = t.first + rr / group, qh = head * group + rr % group;
-                float o[DIM / 32], mm, ll;
-                attend_row_exact<T, DIM>(p, t.seq, tok, rr / group, qh, t.key_lo + s0 * kKeys, t.key_lo + s1 * kKeys, o, mm, ll);
-                if (all) {
-                    const int64_t at = static_cast<int64_t>(tok) * p.a.q_heads + qh;
-                    for (int c = 0; c < DIM / 32; ++c)
-                        from_f32(o[c] * row_inverse(ll), static_cast<T*>(p.a.out)[at * DIM + lane * (DIM / 32) + c]);
-                    if (p.a.lse && lane == 0) p.a.lse[at] = row_lse(mm, ll);
-                } else {
-                    const int64_t at = slot * kRows + rr - t.row0;
-                    for (int c = 0; c < DIM / 32; ++c) r.part[at * DIM + lane * (DIM / 32) + c] = o[c];
-                    if (lane == 0)
-                        *reinterpret_cast<float2*>(r.part + 2ll * r.runs * kRows * DIM + at * 2) = make_float2(mm, ll);
-                }
-            }
+            if (__any_sync(0xffffffffu, *nan_seen))   // by this item or one before: each row gets its NaN back
+                restore_nan<T, DIM>(r, t, head, s0, s1, 128 * h + mine, live, all ? -1 : slot);
         }
         if (!ok && lane == 0) kv_flag(p.c.status, B3_KV_TIMEOUT);
     }

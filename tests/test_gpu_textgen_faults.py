@@ -72,3 +72,89 @@ def test_one_page_table_row_for_all(pkg, max_q):
         c.append(x[:, :4], x[:, 4:6], x[:, 6:], i32(0, 3, 3), i32(20, 150), t)
         c.check()
     assert torch.equal(a.k.view(torch.uint8), b.k.view(torch.uint8)) and torch.equal(a.v_scale, b.v_scale)
+
+
+# ───────────────────────────── NaN in the cache ─────────────────────────────
+
+def ms(f, n=5):
+    f()
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    a.record()
+    for _ in range(n):
+        f()
+    b.record()
+    b.synchronize()
+    return a.elapsed_time(b) / n
+
+
+# dtype, q_heads, kv_heads, dim, page, past, new, causal, window
+NAN_CASES = [
+    (torch.float16, 8, 2, 128, 64, [1900, 30], [300, 500], True, 0),
+    (torch.bfloat16, 6, 2, 64, 16, [700, 0, 90], [200, 333, 1], True, 90),
+    (torch.float16, 2, 2, 128, 32, [100, 1000], [400, 130], True, 300),
+    (torch.bfloat16, 4, 4, 64, 128, [500, 3], [100, 60], False, 0),
+    (torch.float16, 8, 2, 128, 64, [4000, 70, 0, 200], [4, 3, 2, 1], True, 0),
+    (torch.bfloat16, 6, 2, 64, 16, [3000, 5, 90], [5, 2, 4], True, 40),
+    (torch.float16, 16, 1, 128, 32, [900, 20], [1, 1], True, 0),
+    (torch.float16, 4, 2, 64, 32, [900, 20], [6, 8], False, 0),
+]
+
+
+@pytest.mark.parametrize("case", NAN_CASES)
+def test_nan_values_reach_exactly_who_sees_them(pkg, case):
+    """NaN codes of V all over the cache, many among the new tokens: a channel of a
+    row is NaN where a key that it sees has NaN there, everything else keeps its bits."""
+    dtype, q_heads, kv_heads, dim, page, past, new, causal, window = case
+    rng = np.random.default_rng(dim + page + sum(past))
+    dev, cu, kv, table, pages = make_batch(rng, page, past, new)
+    cache = random_cache(pkg, rng, pages, kv_heads, page, dim)
+    q = torch.from_numpy(rng.normal(0, 1, (int(cu[-1]), q_heads, dim)).astype(np.float32)).to(dtype).cuda()
+    call = lambda: cache.attend(q, **dev, max_q=max(new), scale=0.02, causal=causal, window=window, return_lse=True)
+    want, want_lse = call()
+    raw = cache.v.view(torch.uint8)
+    nan_at = [np.zeros((n, kv_heads, dim), bool) for n in kv]
+    for i, n in enumerate(kv):
+        at = np.concatenate([rng.integers(0, n, 3), n - 1 - rng.integers(0, min(n, new[i] + 5), 6)])
+        for j in at:
+            h, c = rng.integers(kv_heads), rng.integers(dim)
+            nan_at[i][j, h, c] = True
+            raw[table[i, j // page], h, j % page, c] = 0x7F if rng.random() < 0.5 else 0xFF
+    got, lse = call()
+    cache.check()
+    expect = np.zeros((int(cu[-1]), q_heads, dim), bool)
+    for i in range(len(kv)):
+        for t in range(new[i]):
+            pos = kv[i] - new[i] + t
+            hi = pos + 1 if causal else kv[i]
+            lo = max(0, pos + 1 - window) if causal and window else 0
+            expect[cu[i] + t] = np.repeat(nan_at[i][lo:hi].any(0), q_heads // kv_heads, 0)
+    bad = torch.isnan(got).cpu().numpy()
+    assert np.array_equal(bad, expect)
+    assert torch.equal(got[~torch.isnan(got)], want[~torch.isnan(got)])
+    assert torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("n,past", [(2048, 14336), (4, 30000)])
+def test_nan_costs_no_more_than_numbers(pkg, n, past):
+    """NaN that rows do see (an early value, a whole padded query) leaves a call's time as it is."""
+    rng = np.random.default_rng(n)
+    page, dim, kv_heads, q_heads = 64, 128, 2, 8
+    dev, cu, kv, table, pages = make_batch(rng, page, [past, 500], [n, n])
+    cache = random_cache(pkg, rng, pages, kv_heads, page, dim)
+    q = torch.from_numpy(rng.normal(0, 1, (int(cu[-1]), q_heads, dim)).astype(np.float32)).half().cuda()
+    call = lambda: cache.attend(q, **dev, max_q=n, scale=0.02)
+    clean = ms(call)
+    want = call()
+    cache.v.view(torch.uint8)[table[0, 0], 1, 3, 7] = 0x7F
+    q[1] = math.nan
+    slow = ms(call)
+    got = call()
+    cache.check()
+    bad = torch.isnan(got)
+    group = q_heads // kv_heads
+    assert bad[1].all() and bad[:n, group:, 7].all()
+    expect = torch.zeros_like(bad)
+    expect[1] = True
+    expect[:n, group:, 7] = True
+    assert torch.equal(bad, expect) and torch.equal(got[~bad], want[~bad])
+    assert slow <= 3 * clean + 0.05, (slow, clean)
