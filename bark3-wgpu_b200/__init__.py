@@ -20,9 +20,12 @@ every entry point raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import pathlib
 import subprocess
+import sys
+import sysconfig
 
 import numpy as np
 
@@ -55,9 +58,13 @@ _lib = None
 
 
 def build(force: bool = False) -> pathlib.Path:
-    """Compile libbark3_b200.so (nvcc, sm_100a) and the torch side of text generation in place."""
-    if force or not LIB_PATH.exists() or not (PKG_DIR / "_textgen.so").exists():
-        subprocess.run(["make", "-C", str(PKG_DIR), "-j8"], check=True)
+    """Compile libbark3_b200.so (nvcc, sm_100a) in place and, where this interpreter
+    has torch, the torch side of text generation for it."""
+    targets = {"libbark3_b200.so": LIB_PATH}
+    if importlib.util.find_spec("torch"):
+        targets["textgen"] = PKG_DIR / f"_textgen{sysconfig.get_config_var('EXT_SUFFIX')}"
+    if force or not all(path.exists() for path in targets.values()):
+        subprocess.run(["make", "-C", str(PKG_DIR), "-j8", f"PYTHON={sys.executable}", *targets], check=True)
     return LIB_PATH
 
 

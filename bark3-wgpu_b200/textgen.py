@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import ctypes
 
-from . import B3_EINVAL, B3_ETIMEOUT, B3Error, lib
+from . import B3_EINVAL, B3_ESTATE, B3_ETIMEOUT, PKG_DIR, B3Error, lib
 
 _P, _I32, _I64, _F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
@@ -58,7 +58,11 @@ def _load():
     """The torch side of the calls (csrc/textgen_ext.cpp), bound to the C ABI."""
     import torch  # noqa: F401  (its libraries are what the extension links to)
 
-    from . import _textgen
+    try:
+        from . import _textgen
+    except ImportError as e:
+        raise B3Error(B3_ESTATE, f"the torch side of text generation is not built for this interpreter "
+                                 f"(run make -C {PKG_DIR} textgen): {e}") from e
 
     L = lib()
     names = ("b3_kv_append", "b3_kv_attend_workspace", "b3_kv_attend", "b3_sample", "b3_last_error")
