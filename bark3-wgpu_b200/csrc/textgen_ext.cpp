@@ -11,8 +11,11 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/core/GradMode.h>
 
+#include <initializer_list>
 #include <string>
+#include <utility>
 
 #include "../../include/bark3_b200.h"
 
@@ -49,6 +52,15 @@ std::string describe(const at::Tensor& t) {
 const at::Tensor& tensor(PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) raise(B3_EINVAL, std::string(name) + " must be a torch tensor");
     return THPVariable_Unpack(o);
+}
+
+// These calls have no backward: where a gradient would be lost, it is said.
+void no_gradient(const char* call, std::initializer_list<std::pair<const char*, PyObject*>> inputs) {
+    if (!c10::GradMode::is_enabled()) return;
+    for (const auto& [name, o] : inputs)
+        if (o && o != Py_None && THPVariable_Check(o) && THPVariable_Unpack(o).requires_grad())
+            raise(B3_EINVAL, std::string(call) + " has no backward and " + name +
+                                 " requires a gradient: call it under torch.no_grad(), or detach " + name);
 }
 
 bool on(const at::Tensor& t, int device) { return t.is_cuda() && t.get_device() == device; }
@@ -116,7 +128,7 @@ void call(int device, F f) {
 template <typename F>
 PyObject* guarded(F f) {
     try {
-        const at::AutoDispatchBelowADInplaceOrView below;   // plain memory: nothing here is differentiated
+        const at::AutoDispatchBelowADInplaceOrView below;   // plain memory: nothing here is differentiated (no_gradient)
         return f();
     } catch (const Raised&) {
     } catch (const std::exception& e) {
@@ -203,6 +215,7 @@ PyObject* cache_append(PyObject* o, PyObject* args, PyObject* kwargs) {
         !ready(self))
         return nullptr;
     return guarded([&]() -> PyObject* {
+        no_gradient("append", {{"q", q_}, {"k", k_}, {"v", v_}, {"q_norm", qn}, {"k_norm", kn}, {"cos", cos}, {"sin", sin}});
         const at::Tensor &q = tensor(q_, "q"), &k = tensor(k_, "k"), &v = tensor(v_, "v");
         const int device = self->device, dim = self->c.head_dim;
         b3_kv_append_args a{};
@@ -261,6 +274,7 @@ PyObject* cache_attend(PyObject* o, PyObject* args, PyObject* kwargs) {
         return nullptr;
     }
     return guarded([&]() -> PyObject* {
+        no_gradient("attend", {{"q", q_}});
         const at::Tensor& q = tensor(q_, "q");
         const int device = self->device;
         b3_kv_attend_args a{};
@@ -306,6 +320,7 @@ PyObject* sample(PyObject*, PyObject* args, PyObject* kwargs) {
     if (!PyArg_ParseTupleAndKeywords(args, kwargs, "OO|$OOOO:sample", const_cast<char**>(names), &x_, &u, &t, &k, &p, &m))
         return nullptr;
     return guarded([&]() -> PyObject* {
+        no_gradient("sample", {{"logits", x_}});
         const at::Tensor& x = tensor(x_, "logits");
         b3_sample_args a{};
         a.dtype = dtype_of(x);

@@ -11,7 +11,8 @@ torch's current stream of that GPU and return; they can be captured in a CUDA
 graph.  What they compute is written down at b3_kv_cache, b3_kv_append,
 b3_kv_attend and b3_sample in include/bark3_b200.h; a bad argument raises
 B3Error(B3_EINVAL), lengths or page numbers that only the GPU sees are reported
-by KvCache.check().
+by KvCache.check().  The calls have no backward: an input that requires a
+gradient is refused unless gradients are off (torch.no_grad()).
 """
 from __future__ import annotations
 

@@ -158,3 +158,33 @@ def test_nan_costs_no_more_than_numbers(pkg, n, past):
     expect[:n, group:, 7] = True
     assert torch.equal(bad, expect) and torch.equal(got[~bad], want[~bad])
     assert slow <= 3 * clean + 0.05, (slow, clean)
+
+
+# ──────────────────────────────── gradients ────────────────────────────────
+
+def test_a_gradient_that_would_be_lost_is_refused(pkg):
+    cache = pkg.KvCache(2, 1, 64, 16)
+    x = torch.ones(1, 3, 64, dtype=torch.float16, device="cuda")
+    w, t = torch.ones(64, device="cuda"), torch.ones(4, 32, device="cuda")
+    b = dict(cu_q=i32(0, 1), kv_lens=i32(1), page_table=i32(0).reshape(1, 1))
+    logits, u = torch.zeros(1, 100, device="cuda"), torch.zeros(1, device="cuda")
+    leaf = lambda a: a.clone().requires_grad_()
+
+    def calls(f):
+        yield "q requires", lambda: cache.append(f(x[:, :1]), x[:, 1:2], x[:, 2:], **b)
+        yield "k requires", lambda: cache.append(x[:, :1], f(x[:, 1:2]), x[:, 2:], **b)
+        yield "v requires", lambda: cache.append(x[:, :1], x[:, 1:2], f(x[:, 2:]), **b)
+        yield "k_norm requires", lambda: cache.append(x[:, :1], x[:, 1:2], x[:, 2:], **b, q_norm=w, k_norm=f(w))
+        yield "cos requires", lambda: cache.append(x[:, :1], x[:, 1:2], x[:, 2:], **b, cos=f(t), sin=t)
+        yield "q requires", lambda: cache.attend(f(x), **b, max_q=1)
+        yield "logits requires", lambda: pkg.sample(f(logits), u)
+
+    for text, call in calls(leaf):
+        with pytest.raises(pkg.B3Error, match=text) as ei:
+            call()
+        assert ei.value.code == pkg.B3_EINVAL
+        with torch.no_grad():
+            call()
+    for _, call in calls(lambda a: leaf(a).detach()):
+        call()
+    cache.check()
