@@ -114,8 +114,9 @@ class KvCache(_ext.Cache):
         self.device = k.device
 
     def check(self) -> None:
-        """Waits for the GPU and raises for what the calls since the last
-        check met that only the GPU could see."""
+        """Waits for the GPU, all its streams, and raises for what the calls
+        since the last check met that only the GPU could see."""
+        _torch.cuda.synchronize(self.device)
         bits = int(self._status.item())
         if not bits:
             return

@@ -188,3 +188,20 @@ def test_a_gradient_that_would_be_lost_is_refused(pkg):
     for _, call in calls(lambda a: leaf(a).detach()):
         call()
     cache.check()
+
+
+# ──────────────────────────────── the status ────────────────────────────────
+
+def test_check_waits_for_other_streams(pkg):
+    """A call that is still waiting on another stream is in what check() reports."""
+    cache = pkg.KvCache(2, 1, 64, 16)
+    x = torch.ones(1, 3, 64, dtype=torch.float16, device="cuda")
+    b = dict(cu_q=i32(0, 1), kv_lens=i32(1), page_table=i32(5).reshape(1, 1))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)
+        cache.append(x[:, :1], x[:, 1:2], x[:, 2:], **b)
+    with pytest.raises(pkg.B3Error, match="page number"):
+        cache.check()
+    cache.check()
