@@ -236,7 +236,11 @@ __device__ __forceinline__ void q_rows(const AppendParams& p, int warp_id) {
     }
     const int s = kv_seq_of(p.b, token);
     int first, begin, end;
-    if (!seq_span(p, s, first, begin, end) || token - first < 0 || token - first >= end - begin) return;
+    if (!seq_span(p, s, first, begin, end)) return;
+    if (token < first || token - first >= end - begin) {   // a row that cu_q gives to no sequence
+        kv_flag(p.c.status, B3_KV_BAD_LENGTH);
+        return;
+    }
     Angles g;
     float2 w[4];
     load_angles<DIM, PAIRED>(g, l, token_position(p, token, begin + token - first), p);

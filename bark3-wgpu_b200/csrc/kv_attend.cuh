@@ -62,6 +62,15 @@ __device__ __forceinline__ SeqSpan attend_span(const AttendParams& p, int s) {
     return r;
 }
 
+// Flags a cu_q that does not lead from 0 to the number of tokens without a step
+// back: some rows would be nobody's, or two sequences'.  By `threads` threads.
+__device__ __forceinline__ void check_cu_q(const AttendParams& p, int thread, int threads) {
+    for (int s = thread; s < p.b.n_seq; s += threads) {
+        const int a = __ldg(p.b.cu_q + s), b = __ldg(p.b.cu_q + s + 1);
+        if (a > b || (s == 0 && a != 0) || (s == p.b.n_seq - 1 && b != p.b.tokens)) kv_flag(p.c.status, B3_KV_BAD_LENGTH);
+    }
+}
+
 // The keys [lo, hi) that new token i of a sequence sees.
 __device__ __forceinline__ void seen_keys(const AttendParams& p, const SeqSpan& s, int i, int& lo, int& hi) {
     lo = 0;

@@ -638,6 +638,7 @@ __global__ void __launch_bounds__(kJoinMax * 32) k_attend_join(const __grid_cons
     const int w0 = static_cast<int>((begin + kItem) / run), w1 = static_cast<int>((begin + units - 1) / run);
     const int slot0 = begin > w0 * run ? 1 : 0;
     const SeqSpan sp = attend_span(p, r.seq0 + seq);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && r.seq0 == 0) check_cu_q(p, threadIdx.x, blockDim.x);
     pdl_wait();   // the partial results are complete (and this kernel ends after the one before it)
     if (units == 0 || w0 == w1) return;
 

@@ -719,6 +719,8 @@ template <typename T, int DIM>
 __global__ void __launch_bounds__(256) k_attend_tiles_join(const __grid_constant__ TilesParams r) {
     constexpr int kPer = DIM / 32;
     const AttendParams& p = r.p;
+    // beside the tiles; inputs of the call, which were there before its first kernel
+    if (blockIdx.x == 0 && blockIdx.y == 0) check_cu_q(p, threadIdx.x, blockDim.x);
     pdl_wait();
     const int heads = p.c.kv_heads, group = p.a.q_heads / heads;
     const int64_t total = __ldg(&r.tile[r.tiles].begin) * heads, run = run_length(total, r.runs);

@@ -295,7 +295,7 @@ typedef struct b3_kv_cache {
  * new tokens, or (attention only) no tokens at all.  Sequences may share pages
  * that are only read; a page that receives tokens belongs to one of them. */
 typedef struct b3_kv_batch {
-    const int32_t* cu_q;        /* [n_seq + 1], cu_q[0] = 0, cu_q[n_seq] = tokens */
+    const int32_t* cu_q;        /* [n_seq + 1], never falling, cu_q[0] = 0, cu_q[n_seq] = tokens */
     const int32_t* kv_lens;     /* [n_seq], the new tokens included */
     const int32_t* page_table;  /* [n_seq][table_stride], table_width entries in use */
     int64_t table_stride;       /* at least table_width, or 0: one row for all sequences */

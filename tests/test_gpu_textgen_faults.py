@@ -205,3 +205,20 @@ def test_check_waits_for_other_streams(pkg):
     with pytest.raises(pkg.B3Error, match="page number"):
         cache.check()
     cache.check()
+
+
+@pytest.mark.parametrize("max_q", [1, 40])
+@pytest.mark.parametrize("cu", [(1, 2, 3), (0, 1, 2), (0, 2, 1, 3), (0, 0, 0)])
+def test_rows_of_no_sequence_are_reported(pkg, cu, max_q):
+    """Three rows, and a cu_q that leaves some of them out, or steps back: their outputs are not written."""
+    cache = pkg.KvCache(8, 1, 64, 16)
+    x = torch.ones(3, 3, 64, dtype=torch.float16, device="cuda")
+    n = len(cu) - 1
+    b = dict(cu_q=i32(*cu), kv_lens=i32(*[20] * n), page_table=torch.arange(2 * n, dtype=torch.int32, device="cuda").reshape(n, 2))
+    cache.attend(x, **b, max_q=max_q)
+    with pytest.raises(pkg.B3Error, match="cu_q"):
+        cache.check()
+    if list(cu) == sorted(cu):
+        cache.append(x[:, :1], x[:, 1:2], x[:, 2:], **b)
+        with pytest.raises(pkg.B3Error, match="cu_q"):
+            cache.check()
