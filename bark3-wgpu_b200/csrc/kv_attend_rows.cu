@@ -442,6 +442,8 @@ __global__ void __launch_bounds__(Cfg<DIM, ROWS>::kWarps * 32, 1)
             ++used;
             if (!ok) {
                 kv_flag(p.c.status, B3_KV_TIMEOUT);
+                // the block must not leave before its copies have landed: this one and those behind it, each with the same limit
+                for (uint32_t u = used - 1; u != issued; ++u) mbar_wait(bars + 8 * (u % C::kStages), (u / C::kStages) & 1, 0x61);
                 break;
             }
 

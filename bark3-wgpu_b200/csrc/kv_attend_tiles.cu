@@ -285,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
     auto p_half = [&](int h) { return bars + 96 + 8 * h; };
     auto p_full = [&](int h) { return bars + 112 + 8 * h; };
     auto o_full = [&](int h) { return bars + 128 + 8 * h; };
+    const uint32_t drained = bars + 144;   // after a wait that ran out: every product issued is done
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kBar + 160);
     // set when NaN codes of V have gone into a product as 0: before v_full of their block, read behind o_full
     volatile uint32_t* nan_seen = reinterpret_cast<uint32_t*>(smem + C::kBar + 164);
@@ -301,6 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
             mbar_init(p_full(i), 4);
             mbar_init(o_full(i), 1);
         }
+        mbar_init(drained, 1);
         fence_mbar_init();
     }
     if (warp == kMmaWarp) {
@@ -378,7 +380,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_tiles(const __grid_const
                     }
                 }
             } while (ok && w.next());
-            if (!ok) kv_flag(p.c.status, B3_KV_TIMEOUT);
+            if (!ok) {
+                kv_flag(p.c.status, B3_KV_TIMEOUT);
+                // products in flight still read and write the memory that the block gives back
+                mma_commit(drained);
+                mbar_wait(drained, 0, 0x7A);
+            }
         }
     } else if (warp >= kExpWarp0) {
         // ── codes to f16 operands ──
