@@ -211,7 +211,8 @@ __device__ __forceinline__ bool seq_span(const AppendParams& p, int s, int& firs
     const int n = __ldg(p.b.cu_q + s + 1) - first;
     end = __ldg(p.b.kv_lens + s);
     begin = end - n;
-    const bool fits = first >= 0 && n >= 0 && n <= p.b.tokens - first && begin >= 0 &&
+    // n <= end and not begin >= 0: of a length near -2^31 the difference would wrap around to a large one
+    const bool fits = first >= 0 && n >= 0 && n <= p.b.tokens - first && n <= end &&
                       end <= static_cast<int64_t>(p.b.table_width) * p.c.page_tokens;
     if (!fits) kv_flag(p.c.status, B3_KV_BAD_LENGTH);
     return fits;

@@ -222,3 +222,13 @@ def test_rows_of_no_sequence_are_reported(pkg, cu, max_q):
         cache.append(x[:, :1], x[:, 1:2], x[:, 2:], **b)
         with pytest.raises(pkg.B3Error, match="cu_q"):
             cache.check()
+
+
+@pytest.mark.parametrize("length", [-1, 0, -(1 << 31), 1 - (1 << 31), (1 << 31) - 1])
+def test_append_lengths_far_out_of_range(pkg, length):
+    cache = pkg.KvCache(4, 1, 64, 16)
+    x = torch.ones(2, 3, 64, dtype=torch.float16, device="cuda")
+    cache.append(x[:, :1], x[:, 1:2], x[:, 2:], i32(0, 2), i32(length), i32(0, 1).reshape(1, 2))
+    with pytest.raises(pkg.B3Error, match="kv_lens"):
+        cache.check()
+    assert not cache.k.float().any() and not cache.v.float().any()
