@@ -472,8 +472,10 @@ int kv_check(const b3_kv_cache* c, const b3_kv_batch* b) {
     if (b->n_seq <= 0 || b->tokens < 0 || b->table_width <= 0 || (b->table_stride < b->table_width && b->table_stride != 0))
         return set_error(B3_EINVAL, "batch of %d sequences, %d tokens, page table %d wide with stride %lld", b->n_seq,
                          b->tokens, b->table_width, static_cast<long long>(b->table_stride));
-    if (static_cast<int64_t>(b->table_width) * c->page_tokens > 0x7fffffffll)
-        return set_error(B3_EINVAL, "a page table of %d entries passes 2^31 tokens", b->table_width);
+    // what is left up to 2^31 lets the kernels round a token's place up to a block or a tile
+    if (static_cast<int64_t>(b->table_width) * c->page_tokens > kMostTokens)
+        return set_error(B3_EINVAL, "a page table of %d entries passes %lld tokens", b->table_width,
+                         static_cast<long long>(kMostTokens));
     return 0;
 }
 

@@ -12,7 +12,7 @@
 namespace b3 {
 
 constexpr int kScaleExpLo = -40, kScaleExpHi = 40;   // 2^e of a page's scale
-constexpr float kE4m3Max = 448.f;
+constexpr int64_t kMostTokens = 0x7fffffff - 1023;   // of a sequence
 
 // Checks of b3_kv_cache / b3_kv_batch that the host can make (kv_append.cu).
 int kv_check(const b3_kv_cache* c, const b3_kv_batch* b);

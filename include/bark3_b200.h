@@ -299,7 +299,7 @@ typedef struct b3_kv_batch {
     const int32_t* kv_lens;     /* [n_seq], the new tokens included */
     const int32_t* page_table;  /* [n_seq][table_stride], table_width entries in use */
     int64_t table_stride;       /* at least table_width, or 0: one row for all sequences */
-    int32_t table_width;
+    int32_t table_width;        /* table_width * page_tokens <= 2^31 - 1024 */
     int32_t n_seq;
     int32_t tokens;
 } b3_kv_batch;

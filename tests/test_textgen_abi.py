@@ -107,3 +107,14 @@ def test_append_attend_and_sample_are_checked(pkg, structs):
     assert L.b3_sample(None, None) == pkg.B3_EINVAL
     smp.rows = 0
     assert L.b3_sample(ref(smp), None) == 0
+
+
+def test_a_sequence_of_nearly_two_to_the_31_tokens_is_refused(pkg, structs):
+    """Past 2^31 - 1024 tokens a place rounded up to a kernel's block would leave 32 bits."""
+    p, cache, batch, app, att, smp, _ = structs
+    L = pkg.lib()
+    batch.table_width = batch.table_stride = (1 << 31) // cache.page_tokens - 63
+    for rc in (L.b3_kv_append(ref(cache), ref(batch), ref(app), None),
+               L.b3_kv_attend(ref(cache), ref(batch), ref(att), None, 0, None),
+               L.b3_kv_attend_workspace(ref(cache), ref(batch), ref(att))):
+        assert rc == pkg.B3_EINVAL and "2147482624 tokens" in pkg.last_error()
