@@ -66,8 +66,8 @@ struct Cfg {
 struct RowsParams {
     AttendParams p;
     int seq0, seqs;        // this launch's sequences
-    int workers, rows;     // warps of the grid; row capacity of a partial result (8 or 16)
-    float* part;           // [workers][2][rows][DIM] outputs, then [workers][2][rows][2] (m, l)
+    int workers;           // warps of the grid
+    float* part;           // [workers][2][ROWS][DIM] outputs, then [workers][2][ROWS][2] (m, l)
 };
 
 // Score row c (0..7) of a tile's half stands for this key of the half's eight.
@@ -721,7 +721,7 @@ int launch(const AttendParams& p, void* workspace, cudaStream_t st) {
     rc = make_map_2d(&mk, p.c.k, kMapU8, 128, lines, 128, 128, box, true);
     if (!rc) rc = make_map_2d(&mv, p.c.v, kMapU8, 128, lines, 128, 128, box, true);
     if (rc) return rc;
-    RowsParams r{p, 0, 0, workers_of<DIM>(ROWS), ROWS, static_cast<float*>(workspace)};
+    RowsParams r{p, 0, 0, workers_of<DIM>(ROWS), static_cast<float*>(workspace)};
     // sequences a launch: the prefix array's room, and all their units in 31 bits
     const int64_t most = static_cast<int64_t>(p.b.table_width) * p.c.page_tokens / kStep + 2 + kItem;
     const int at_once = static_cast<int>(std::min<int64_t>(kMaxSeqs, 0x7fffffffll / most));

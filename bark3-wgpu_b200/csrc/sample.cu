@@ -148,7 +148,6 @@ struct Row {
     bool by_one;           // values one by one: off is 0 wherever the row starts
     // place of value e: index + off
     __device__ __forceinline__ int index(int e) const { return base + (e / kVec) * 32 * kVec + e % kVec - off; }
-    __device__ __forceinline__ float at(int i) const { return to_f32(x[i]); }
 
     // The thread's values into its column, their maximum; what is no number, or outside the row, is -inf.
     __device__ __forceinline__ float load(uint4* col) const {
