@@ -427,12 +427,16 @@ int launch_dim(AppendParams& p, cudaStream_t st) {
                          static_cast<long long>(p.b.tokens));
     p.kv_blocks = static_cast<int>(kv_blocks);
     if (!whole) return launch<T, DIM, VEC, PAIRED, 1, 0>(p, blocks, st);
+    // pages of 16 to 128 tokens: 1 to 8 passes of 16 rows of 128 channels, 0 to 4 of 32 rows of 64
+    if constexpr (DIM == 128) {
+        if (passes == 8) return launch<T, DIM, VEC, PAIRED, kWarps, 8>(p, blocks, st);
+    } else {
+        if (passes == 0) return launch<T, DIM, VEC, PAIRED, 4, 1>(p, blocks, st);
+    }
     switch (passes) {
-        case 8: return launch<T, DIM, VEC, PAIRED, kWarps, 8>(p, blocks, st);
         case 4: return launch<T, DIM, VEC, PAIRED, kWarps, 4>(p, blocks, st);
         case 2: return launch<T, DIM, VEC, PAIRED, kWarps, 2>(p, blocks, st);
-        case 1: return launch<T, DIM, VEC, PAIRED, kWarps, 1>(p, blocks, st);
-        default: return launch<T, DIM, VEC, PAIRED, 4, 1>(p, blocks, st);
+        default: return launch<T, DIM, VEC, PAIRED, kWarps, 1>(p, blocks, st);
     }
 }
 
