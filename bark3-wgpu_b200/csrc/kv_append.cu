@@ -4,27 +4,36 @@
 //   x' = R(pos) (x / sqrt(mean(x^2) + eps) * w)     for each head of q and k
 //   q_out = round16(q'),  k' and v' = v -> code = e4m3(x' / 2^e), scale 2^e
 // with e of a (page, head) from the largest finite magnitude that the page
-// holds.  Bound by memory: each value is read once and leaves as two bytes
-// (q) or one (k, v); the arithmetic is some ten operations a value.
+// holds.  Bound by memory: each value leaves as two bytes (q) or one (k, v)
+// and is read once, but for pages that one warp fills by many rows (GROUP = 1
+// below); the arithmetic is some ten operations a value.
 //
 // One launch.  The first blocks own the cache: a (page, key head, k or v) that
 // receives tokens belongs to one group of warps, which finds the page's new
-// exponent over all its new rows before it writes a code, so no atomics and no
-// second pass over memory order the scale.  The other blocks own q, a few
-// heads of a token for each warp.  A row of head_dim channels is held by
+// exponent over all its new rows before it writes a code, so no atomics order
+// the scale.  The other blocks own q, 8 heads of 128 channels (16 of 64) of a
+// token for each warp.  A row of head_dim channels is held by
 // head_dim / 8 lanes, eight channels each; the norm's sum by shuffles within
 // the row.  PAIRED (the usual rotation of all channels, i with i + head_dim / 2)
 // gives a lane four channels and their four partners, so the rotation stays in
 // the lane; otherwise a lane has eight neighbours and shuffles for partners.
-//   GROUP = 1     a warp a (page, head).  Decode brings one row to each page.
+//   GROUP = 1     a warp a (page, head).  Decode brings one row to each page;
+//                 more rows than 256 / head_dim are read, normed and turned
+//                 again after the exponent is known.
 //   GROUP = 4, 8  that many warps, the page's rows in registers between the
 //                 exponent and the codes.  Prompts fill whole pages; four warps
 //                 hold 16 rows of 64 channels.
-// The host takes groups from four new tokens a sequence on average.
+// The host takes groups from four new tokens a sequence on average: one choice
+// for the call, so of a mixed batch one part goes the wrong way (32 + 2 x 8 heads
+// of 128 in bf16: 127 sequences of one token 4.0 us, a prompt of 512 tokens 5.1,
+// both in one call, in groups, 24; 255 sequences 5.8, a prompt of 700 5.1, both
+// by single warps 44).
 //
 // Measured: 16384 tokens of 32 + 2 x 8 heads of 128 in bf16 84 us (378 MB at
-// 4.5 TB/s); one token for each of 256 sequences of the same heads 5.8 us, where
-// the launch and three dependent loads (lengths, page, row) set the time.
+// 4.5 TB/s), 29 of 64 warps resident at 64 registers, most often waiting for
+// loads; one token for each of 256 sequences of the same heads
+// 5.7 us: the launch, then loads one behind the other (lengths, page number and,
+// behind the page's check though its address does not need it, the row).
 #include "kv_cache.cuh"
 
 namespace b3 {

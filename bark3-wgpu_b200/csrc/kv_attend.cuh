@@ -13,6 +13,14 @@
 //   p'_ij = 2^(x'_ij - m) <= 1  (f16 for the product),   o = sum p' vc / l,
 //   l = sum p' 2^-ve = sum 2^(x_ij - m).
 // With ve in [-40, 40] a p' that underflows f32 has a share below 2^-46 of l.
+//
+// p' is rounded to f16 for the second product, l is summed from the unrounded
+// ones.  f16 keeps 2^-11 of a p' down to 2^-14; below that p' is a multiple of
+// 2^-24.  Because p' carries ve, that is where a key's probability times its
+// value page's scale is 2^-14 of the row's largest such product: a page whose
+// scale is so far below another's contributes with an error of up to 2^-25 of
+// the largest product times its codes, whatever its own size.  Operands of more
+// bits would double the tensor cores' work (tf32) for terms that small.
 #pragma once
 #include "kv_cache.cuh"
 

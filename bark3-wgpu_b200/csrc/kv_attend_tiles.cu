@@ -18,10 +18,10 @@
 //                      write P (f16) over them, move the reference maximum only
 //                      when a row's grows by more than 2^8 (and then rescale O
 //                      in TMEM), and store the output.
-//   warps 8..14        expand codes to f16 operands: 16-byte loads of a page's
-//                      rows, one block ahead in registers, K and V both as
-//                      128-byte swizzled rows of 64 channels (K-major for S,
-//                      MN-major for PV).
+//   warps 8..14        expand codes to f16 operands in tasks of 16 keys: 16-byte
+//                      loads of a page's rows two tasks ahead in registers, K
+//                      and V both as 128-byte swizzled rows of 64 channels
+//                      (K-major for S, MN-major for PV).
 //   warp 15            one thread issues S = Q K^T (M128 N128 K128) and
 //                      O += P V (M128 N128 K128, P from TMEM).
 // TMEM: S/P of both halves 2 x 128 columns, O 2 x 128.
@@ -51,7 +51,7 @@ constexpr int kKeys = 128;          // keys of a block
 // 16 warps, four on each scheduler: a 17th would cut every thread's registers from 128 to 96
 constexpr int kThreads = 512;
 constexpr int kExpWarp0 = 8, kExpWarps = 7, kMmaWarp = 15;
-constexpr int kItem = 3;            // what an item's start and end cost, in blocks
+constexpr int kItem = 3;            // what an item's start and end cost, in blocks (measured on prompts of head_dim 64)
 constexpr float kMove = 8.f;        // log2: how far a maximum may pass the reference
 
 struct Tile {

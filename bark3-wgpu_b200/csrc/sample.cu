@@ -13,9 +13,12 @@
 // by it alone; a warp's values are neighbours in the row, in index order over
 // (vector, lane, place)).  Shared memory and not registers: loops over 32
 // values unrolled with an exponential in each miss the instruction cache.
-// Bound by some 57 instructions a value for many rows, by the chain of block-
-// and cluster-wide steps for few.  Measured, settings of each kind mixed: 256 rows
-// x 131072 in 16 bits 124 us (one read takes 10), 256 x 8193 in f32 24, one row 11.
+// Bound by instructions for many rows (55 a value on average, at 0.57 of the
+// issue rate), by the chain of block- and cluster-wide steps for few.  Measured,
+// settings of each kind mixed: 256 rows x 131072 in 16 bits 125 us (one read takes
+// 10), 256 x 8193 in f32 24, one row 11; all rows of one kind, 131072 and 8193:
+// no filter 81 and 11, top-k 50 89 and 13, top-k 5000 173 and 23, top-p 197 and
+// 26, greedy 41 and 6.
 //   top_k <= 512   Each warp's j-th largest thread maximum, j = ceil(k / warps),
 //                  bounds the k-th largest logit from below (the warps hold k
 //                  values that large); what reaches the bound, a few hundred

@@ -341,8 +341,14 @@ int b3_kv_append(const b3_kv_cache* cache, const b3_kv_batch* batch, const b3_kv
  * sequence.  A query that sees no key gives zeros and lse = -inf.  lse is the
  * natural logarithm of the sum of exponentials.  Scores, softmax and sums are
  * f32; the products' operands are the e4m3 codes and 16-bit queries, both
- * exact, and probabilities rounded to f16.
- * `max_q` is an upper bound of the new tokens of any one sequence.
+ * exact, and probabilities rounded to f16 after they have been multiplied by
+ * their value page's scale and divided by the row's largest such product (or
+ * one up to 2^8 below it): where a product is below 2^-14 of the largest the
+ * rounding is 2^-25 of the largest.  A NaN key or value reaches the rows that see it
+ * and no others.
+ * `max_q` is an upper bound of the new tokens of any one sequence; with
+ * max_q * (q_heads / kv_heads) <= 16 the kernel for few rows runs, so a batch
+ * that decodes and a prompt are faster as two calls than as one.
  * `workspace` (16-byte aligned, b3_kv_attend_workspace bytes) is scratch of
  * this call alone: calls that may overlap need one each. */
 typedef struct b3_kv_attend_args {
