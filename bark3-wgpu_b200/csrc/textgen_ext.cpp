@@ -5,6 +5,7 @@
 //
 // In C++ because a decode step's calls are short: checking a dozen tensors and
 // making the call took 15 us of Python around 3 to 5 us of launches.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
@@ -13,6 +14,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <c10/core/GradMode.h>
 
+#include <exception>
 #include <initializer_list>
 #include <string>
 #include <utility>
@@ -131,8 +133,8 @@ PyObject* guarded(F f) {
         const at::AutoDispatchBelowADInplaceOrView below;   // plain memory: nothing here is differentiated (no_gradient)
         return f();
     } catch (const Raised&) {
-    } catch (const std::exception& e) {
-        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {   // torch's own: each as the Python type that torch gives it (out of memory among them)
+        if (!PyErr_Occurred()) torch::translate_exception_to_python(std::current_exception());
     }
     return nullptr;
 }

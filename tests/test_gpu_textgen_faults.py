@@ -232,3 +232,23 @@ def test_append_lengths_far_out_of_range(pkg, length):
     with pytest.raises(pkg.B3Error, match="kv_lens"):
         cache.check()
     assert not cache.k.float().any() and not cache.v.float().any()
+
+
+# ──────────────────────────────── errors ────────────────────────────────
+
+def test_out_of_memory_is_torchs(pkg):
+    """An allocation that fails inside a call raises what torch raises for it, and the cache goes on."""
+    cache = pkg.KvCache(2, 1, 64, 16)
+    n = 4_000_000
+    x = torch.zeros(1, 1, 64, dtype=torch.float16, device="cuda").expand(n, 1, 64)   # an output of half a gigabyte
+    b = dict(cu_q=i32(0, n), kv_lens=i32(3), page_table=i32(0).reshape(1, 1))
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.001)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            cache.attend(x, **b, max_q=n)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    out = cache.attend(x[:2], **{**b, "cu_q": i32(0, 2)}, max_q=2)
+    cache.check()
+    assert out.shape == (2, 1, 64)
